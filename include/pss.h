@@ -186,7 +186,7 @@ int pss_emit_path(pss_sampler *h, int32_t *path);
  *       one decode serves every rank of a call, whatever their number.  A workspace the
  *       device cannot hold makes pss_generate return PSS_EHIP.  After calls for consecutive
  *       epochs of one shape, the MT draws of the next epochs (up to 8) are made ahead on the
- *       handle's own low-priority streams where they are few long streams (shuffle_buffer
+ *       handle's own side streams where they are few long streams (shuffle_buffer
  *       beyond 4096 with few windows), within pss_set_lookahead's bounds (1 GiB of draw slots
  *       by default); pss_destroy waits for them.
  * Replaces nothing in the reference: its order IS the exact one. */
@@ -203,7 +203,7 @@ int pss_order_mode(const pss_sampler *h, int32_t *mode);
  *   exact_max_bytes -- the bytes ALL the exact draw slots together may hold, the one a call is
  *                      reading included (default 1 GiB; 0: none); the depth shrinks to fit;
  *   v2_depth        -- V2 counter order (pools up to 16384): epochs whose last-occurrence pass
- *                      is queued ahead on a low-priority stream (-1: 2, the default; 0: the pass
+ *                      is queued ahead on a side stream (-1: 2, the default; 0: the pass
  *                      runs in line; 1 or 2), each in its own VAL buffer (v2 VAL ring).
  * Slot memory beyond the bounds is released by later calls once idle (no host wait).  The
  * lookaheads are best effort: an error while preparing one (e.g. hipMalloc of a slot) turns

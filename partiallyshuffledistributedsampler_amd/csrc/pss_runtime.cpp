@@ -307,7 +307,7 @@ struct pss_sampler {
     size_t open_ev = 0;
     // V2 epoch lookahead: once generate() has been called with one shape for consecutive epochs,
     // the last-occurrence pass (VAL tables + key table, or the pools-beyond-LDS bucketing
-    // workspace; all depend only on the epoch key and the shape) of epoch e+1 is queued on a low-priority side stream beside epoch e's replay, into the
+    // workspace; all depend only on the epoch key and the shape) of epoch e+1 is queued on a side stream beside epoch e's replay, into the
     // other of two VAL buffers.  generate(e+1) with the same shape then launches the replay only.
     // PSS_V2_LOOKAHEAD=0 turns it off.
     static constexpr int kLaBufs = 3;   // VAL (and big-pool workspace) ring: d_val/d_buf + 2
@@ -335,7 +335,7 @@ struct pss_sampler {
     // Exact-order draw lookahead: the reference's draws depend on the epoch and the windows alone
     // (V1:165-171; V2:107-109,147), so once pss_generate ran in exact order for consecutive
     // epochs of one call shape, the MT draws of the next epochs are made ahead into draw slots,
-    // each on its own low-priority side stream (a few long windows keep ~11 CUs busy for
+    // each on its own side stream (a few long windows keep ~11 CUs busy for
     // milliseconds: several epochs' draws run side by side).  The call of a prepared epoch only
     // decodes (V2) / resolves (V1).  PSS_EXACT_LOOKAHEAD=0 turns it off.
     static constexpr int kXSlots = 9;
@@ -830,11 +830,9 @@ int generate_v2_lookahead(pss_sampler *h, const pss::Geometry &g, int32_t rank_l
         return PSS_OK;
     };
     if (!h->side) {
-        int least = 0, greatest = 0;
-        PSS_HIP(hipDeviceGetStreamPriorityRange(&least, &greatest));
-        // the lowest priority: at the highest the C2 step was slower (519 vs 526 G idx/s, round 2)
-        (void)greatest;
-        PSS_HIP(hipStreamCreateWithPriority(&h->side, hipStreamNonBlocking, least));
+        // the default priority, as every stream here: work on streams of different priorities
+        // can hang the device
+        PSS_HIP(hipStreamCreateWithFlags(&h->side, hipStreamNonBlocking));
         // these events only order device work on this device (never inspected by the host):
         // without the system-scope fence a step takes 176 against 179 us at C2, same box
         // (profiles/r04/ab_evflags; device-scope release alone: 179)
@@ -1012,9 +1010,7 @@ int generate_exact(pss_sampler *h, const pss::Geometry &g, int32_t rank_lo, int3
     auto prepare_slot = [&](int k, int64_t ep) -> hipError_t {
         hipError_t r;
         if (!h->xside[k]) {
-            int least = 0, greatest = 0;
-            if ((r = hipDeviceGetStreamPriorityRange(&least, &greatest)) != hipSuccess) return r;
-            if ((r = hipStreamCreateWithPriority(&h->xside[k], hipStreamNonBlocking, least)) != hipSuccess) return r;
+            if ((r = hipStreamCreateWithFlags(&h->xside[k], hipStreamNonBlocking)) != hipSuccess) return r;
             if ((r = hipEventCreateWithFlags(&h->xev_done[k], PSS_LA_EVENT_FLAGS)) != hipSuccess) return r;
             if ((r = hipEventCreateWithFlags(&h->xev_read[k], PSS_LA_EVENT_FLAGS)) != hipSuccess) return r;
         }

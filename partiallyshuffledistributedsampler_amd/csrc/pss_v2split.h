@@ -853,9 +853,7 @@ static SpSide *sp_side() {
     auto &p = per[dev];
     if (!p) {
         p = std::make_unique<SpSide>();
-        int lo = 0, hi = 0;
-        bool ok = hipDeviceGetStreamPriorityRange(&lo, &hi) == hipSuccess &&
-                  hipStreamCreateWithPriority(&p->g, hipStreamNonBlocking, hi) == hipSuccess &&
+        bool ok = hipStreamCreateWithFlags(&p->g, hipStreamNonBlocking) == hipSuccess &&
                   hipEventCreateWithFlags(&p->start, hipEventDisableTiming) == hipSuccess;
         for (hipEvent_t &e : p->ev) ok = ok && hipEventCreateWithFlags(&e, hipEventDisableTiming) == hipSuccess;
         if (!ok) (void)hipGetLastError();
