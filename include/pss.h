@@ -217,6 +217,86 @@ int pss_workspace_bytes(const pss_sampler *h, int64_t *bytes);
  * [2] V2 passes queued ahead, [3] V2 replays that used one. */
 int pss_lookahead_stats(const pss_sampler *h, int64_t *stats /* [4] */);
 
+/* ---- batch-row operators ------------------------------------------------------------------
+ * What a batch's rows go through between the sampler and a model's experts.  All but
+ * pss_gather_dropout take no handle: they run on the current device (pointers and stream belong
+ * to it), allocate nothing, keep nothing, and calls on different streams are independent.  Rows
+ * are rows of `cols` values of one dtype, adjacent in a row; `ld*` is the distance between rows
+ * in values (0: the same row for all), any alignment the type allows.  Outputs are contiguous. */
+#define PSS_F32 0
+#define PSS_BF16 1
+#define PSS_F16 2
+
+/* Dropout by counter.  The value in column c of a row with id r is kept iff u >= round(p * 65536),
+ * where u is the 16-bit half c % 8 (low half of a word first) of the Philox4x32-10 block with the
+ * counter (c / 8, r mod 2^32, r / 2^32, 6) under `key`; a kept value is multiplied by
+ * 65536 / (65536 - round(p * 65536)), a dropped one is 0 whatever it was.  So p is taken to the
+ * nearest 1/65536, the mean is kept exactly, nothing is stored, and the gradient is the same call
+ * on the gradient.  Row i has the id row0 + i; row0 + row_ids[0] + i with n_ids == 1; row0 +
+ * row_ids[i] with n_ids == rows.  row_ids is read on the device, so a captured call can be replayed
+ * with other ids. */
+/* The key of one epoch's draws of one logical rank (`site`: any number that tells apart the places
+ * of a model that drop): with a row's id = its position in the rank's stream the mask depends
+ * neither on the batch size, nor on where a run resumed, nor on which GPU generates the rank. */
+int pss_dropout_key(uint64_t seed, int64_t epoch, int32_t rank, int32_t site, uint64_t *key);
+/* y[r] = dropout(x[r]) (+ residual[r] if not NULL, added in 32 bits before the one rounding).  y
+ * overlaps neither.  host != 0: every pointer is host memory, the CPU mode (the
+ * same bits). */
+int pss_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows, int64_t cols,
+                int32_t dtype, double p, uint64_t key, int64_t row0, const int64_t *row_ids, int64_t n_ids,
+                int32_t host, void *stream);
+/* pss_gather of rows of row_values values, dropped in the same pass. */
+int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int64_t row_values,
+                       const int64_t *base_rows_dev, const int32_t *file_pos_dev, const int32_t *offset_dev, int64_t n,
+                       double p, uint64_t key, int64_t row0, const int64_t *row_ids_dev, int64_t n_ids, void *out_dev,
+                       void *stream);
+
+/* Routing: the k experts of every row, their weights, and the rows sorted by expert.
+ *   s = softmax(logits of the row) or sigmoid(logit); an expert's choice value is s + bias (bias:
+ *   [experts] or NULL).  groups > 1: consecutive experts form equal groups, a group's value is the
+ *   sum of its group_sum (1 or 2) best choice values, and only the top_groups best groups stay.  The
+ *   k best choice values win, in falling order; equal ones go to the lower index.  Choice values are
+ *   compared as computed in 64 bits; without a bias (and with group_sum 1 or one group) as the
+ *   logits themselves.
+ *   weight = scale * s, over the sum of the chosen s if renorm (the bias is in no weight).
+ *   A logit of -infinity masks the expert.  A row with fewer live experts than k has experts -1 and
+ *   weights 0 at the end, a row with valid[t] == 0 in all slots (its logits are ignored).  A NaN
+ *   counts as the lowest of all live choices, and the weights of its row are NaN.
+ *   offsets[e] = rows of the experts before e, offsets[experts] = rows in all.  Slot s = t * k + j
+ *   has the place pos[s] in the order by (expert, t); slots without an expert come after
+ *   offsets[experts], in their own order; src is the inverse of pos.
+ * experts <= 1024, k <= 16, groups <= 64, tokens * k < 2^31.  ws: pss_route_workspace bytes, used by
+ * this call alone while it runs.  Results do not depend on timing: no order of atomics enters. */
+#define PSS_SOFTMAX 0
+#define PSS_SIGMOID 1
+int64_t pss_route_workspace(int64_t tokens, int32_t experts);
+int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype, int32_t score,
+              const float *bias, const uint8_t *valid, int32_t groups, int32_t top_groups, int32_t group_sum,
+              int32_t renorm, double scale, int32_t *out_experts, float *out_weights, int32_t *offsets, int32_t *pos,
+              int32_t *src, void *ws, int64_t ws_bytes, void *stream);
+/* The weights' gradient dweights [tokens, k] -> dlogits [tokens, experts] (contiguous, every value
+ * written); logits, chosen and weights as pss_route had and gave them. */
+int pss_route_grad(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype,
+                   int32_t score, int32_t renorm, double scale, const int32_t *chosen, const float *weights,
+                   const float *dweights, void *dlogits, void *stream);
+
+/* Rows into expert order: xs[pos[t, j]] = x[t]; 0 where the slot has no expert. */
+int pss_dispatch(const void *x, int64_t ldx, int64_t tokens, int32_t k, int64_t cols, int32_t dtype,
+                 const int32_t *experts, const int32_t *pos, void *xs, void *stream);
+/* Rows back: out[t] = residual[t] + dropout(sum of weights[t, j] * y[pos[t, j]] over the slots with
+ * an expert), summed in 32 bits in the order of j; residual NULL: none, weights NULL: all 1 (that is
+ * the gradient of pss_dispatch). */
+int pss_combine(const void *y, int64_t tokens, int32_t k, int64_t cols, int32_t dtype, const int32_t *experts,
+                const int32_t *pos, const float *weights, const void *residual, int64_t ldr, double p, uint64_t key,
+                int64_t row0, const int64_t *row_ids, int64_t n_ids, void *out, void *stream);
+/* With g = dropout(dout): dy[pos[t, j]] = weights[t, j] * g[t] and dweights[t, j] = <g[t], y[pos[t, j]]>,
+ * both 0 where the slot has no expert; dy or dweights NULL: not wanted.  The residual's gradient is
+ * dout itself. */
+int pss_combine_grad(const void *dout, int64_t ldo, const void *y, int64_t tokens, int32_t k, int64_t cols,
+                     int32_t dtype, const int32_t *experts, const int32_t *pos, const float *weights, double p,
+                     uint64_t key, int64_t row0, const int64_t *row_ids, int64_t n_ids, void *dy, float *dweights,
+                     void *stream);
+
 /* Self-test of the wave64 DPP scan primitive: out_dev[2i] = 64-bit inclusive wave scan,
  * out_dev[2i+1] = 32-bit one (low words), for n inputs. */
 int pss_debug_wave_scan(const uint64_t *in_dev, uint64_t *out_dev, int64_t n, void *stream);

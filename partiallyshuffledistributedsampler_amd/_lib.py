@@ -17,6 +17,7 @@ _c_i64p = ctypes.POINTER(ctypes.c_int64)
 _c_i32p = ctypes.POINTER(ctypes.c_int32)
 _vp = ctypes.c_void_p
 _i32, _i64, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
+_f64 = ctypes.c_double
 
 # name -> (argtypes, restype); kept in sync with include/pss.h (tests check both directions)
 SIGNATURES = {
@@ -55,6 +56,21 @@ SIGNATURES = {
     "pss_set_lookahead": ([_vp, _i32, _i64, _i32], ctypes.c_int),
     "pss_workspace_bytes": ([_vp, _c_i64p], ctypes.c_int),
     "pss_lookahead_stats": ([_vp, _c_i64p], ctypes.c_int),
+    "pss_dropout_key": ([_u64, _i64, _i32, _i32, ctypes.POINTER(_u64)], ctypes.c_int),
+    "pss_dropout": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _f64, _u64, _i64, _vp, _i64, _i32,
+                     _vp], ctypes.c_int),
+    "pss_gather_dropout": ([_vp, _vp, _i32, _i64, _vp, _vp, _vp, _i64, _f64, _u64, _i64, _vp, _i64,
+                            _vp, _vp], ctypes.c_int),
+    "pss_route_workspace": ([_i64, _i32], _i64),
+    "pss_route": ([_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f64,
+                   _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp], ctypes.c_int),
+    "pss_route_grad": ([_vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f64, _vp, _vp, _vp, _vp,
+                        _vp], ctypes.c_int),
+    "pss_dispatch": ([_vp, _i64, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp], ctypes.c_int),
+    "pss_combine": ([_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _f64, _u64, _i64, _vp,
+                     _i64, _vp, _vp], ctypes.c_int),
+    "pss_combine_grad": ([_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _f64, _u64, _i64,
+                          _vp, _i64, _vp, _vp, _vp], ctypes.c_int),
 }
 
 _lib = None

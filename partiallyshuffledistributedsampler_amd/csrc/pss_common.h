@@ -14,7 +14,8 @@
 
 namespace pss {
 
-enum : uint32_t { DOM_V1_WIN = 1, DOM_V2_SLOT = 2, DOM_V2_INS = 3, DOM_V2_TAIL = 4, DOM_V2_INIT = 5 };
+enum : uint32_t { DOM_V1_WIN = 1, DOM_V2_SLOT = 2, DOM_V2_INS = 3, DOM_V2_TAIL = 4, DOM_V2_INIT = 5,
+                DOM_DROPOUT = 6 };
 
 // Philox4x32-10 (Salmon et al., SC'11).  Each 64-bit product is one v_mad_u64_u32 on gfx950.
 PSS_HD void philox4x32_10(uint32_t &c0, uint32_t &c1, uint32_t &c2, uint32_t &c3,

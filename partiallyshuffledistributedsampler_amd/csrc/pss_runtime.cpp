@@ -24,6 +24,7 @@
 #include "pss_host_mt.h"
 #include "pss_cpu.h"
 #include "pss_map.h"
+#include "pss_rows.h"
 
 using pss::CPythonMT;
 
@@ -628,6 +629,10 @@ pss::MapArgs map_args(const pss_sampler *h, int32_t *fpos, int32_t *off) {
 }
 
 }  // namespace
+
+namespace pss {
+int set_error(int code, const char *msg) { return fail(code, msg); }
+}  // namespace pss
 
 extern "C" {
 
@@ -1387,6 +1392,32 @@ int pss_gather(pss_sampler *h, const void *data_dev, int64_t row_bytes, const in
     if (rc) return rc;
     PSS_HIP(pss::launch_gather(data_dev, row_bytes, base_rows_dev, h->tab[h->tab_cur].order, file_pos_dev,
                                offset_dev, n, out_dev, s));
+    return tables_read(h, s);
+}
+
+int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int64_t row_values,
+                       const int64_t *base_rows_dev, const int32_t *file_pos_dev, const int32_t *offset_dev, int64_t n,
+                       double p, uint64_t key, int64_t row0, const int64_t *row_ids_dev, int64_t n_ids, void *out_dev,
+                       void *stream) {
+    if (!h) return fail(PSS_EINVAL, "NULL handle");
+    if (n > 0 && (!base_rows_dev || !file_pos_dev || !offset_dev)) return fail(PSS_EINVAL, "bad arguments");
+    pss::Drop d;
+    int rc = pss::check_rows(data_dev, row_values, out_dev, n, row_values, dtype);
+    if (rc == PSS_OK) rc = pss::make_drop(p, key, row0, row_ids_dev, n_ids, n, &d);
+    if (rc) return rc;
+    if (n == 0 || row_values == 0) return PSS_OK;
+    if (h->cpu) {
+        const pss::RowGather g{base_rows_dev, h->order.data(), file_pos_dev, offset_dev};
+        pss::cpu::dropout(data_dev, row_values, nullptr, 0, out_dev, n, row_values, dtype, d, &g);
+        return PSS_OK;
+    }
+    DeviceGuard dg(h->device);
+    hipStream_t s = (hipStream_t)stream;
+    SharedUse su(h, s);
+    rc = prepare_tables(h, s);
+    if (rc) return rc;
+    const pss::RowGather g{base_rows_dev, h->tab[h->tab_cur].order, file_pos_dev, offset_dev};
+    PSS_HIP(pss::launch_dropout(data_dev, row_values, nullptr, 0, out_dev, n, row_values, dtype, d, &g, s));
     return tables_read(h, s);
 }
 

@@ -160,10 +160,12 @@ class IndexEngine:
                   _stream_ptr(stream, d))
         return fpos, off
 
-    def gather(self, data, base_rows, fpos, off, out=None, stream=None):
+    def gather(self, data, base_rows, fpos, off, out=None, stream=None, p=0.0, key=0, rows=0):
         """Rows of device-resident files (pss_gather): data [rows, ...] holds every dataset file's
         samples, file f starting at row base_rows[f] (dataset order); returns data rows of the
-        (file_pos, offset) pairs, in their order (the on-GPU form of V1:243-248)."""
+        (file_pos, offset) pairs, in their order (the on-GPU form of V1:243-248).
+        p > 0: the rows (float32, bfloat16 or float16) with dropout, in the same pass
+        (pss_gather_dropout) -- exactly ops.dropout(rows flattened to [n, values], p, key, rows)."""
         d = self._dev()
         fpos = fpos.reshape(-1).contiguous()
         off = off.reshape(-1).to(torch.int32).contiguous()
@@ -173,6 +175,20 @@ class IndexEngine:
         row_bytes = data[0].numel() * data.element_size() if data.dim() > 0 and data.shape[0] else 0
         if out is None:
             out = torch.empty((n,) + tuple(data.shape[1:]), dtype=data.dtype, device=d)
+        if p:
+            from .ops import DTYPES, _p, _row_ids
+            if data.dtype not in DTYPES:
+                raise TypeError("gather with dropout needs float32, bfloat16 or float16 data, got %s" % data.dtype)
+            if not (out.is_contiguous() and out.dtype == data.dtype and out.device == d
+                    and out.numel() >= n * (row_bytes // data.element_size())):
+                raise ValueError("gather: out must be contiguous, of the data's dtype, on the engine's device")
+            row0, ids = _row_ids(rows, n, d)
+            _lib.call("pss_gather_dropout", self._h, ctypes.c_void_p(data.data_ptr()), DTYPES[data.dtype],
+                      row_bytes // data.element_size(), ctypes.c_void_p(base_rows.data_ptr()),
+                      ctypes.c_void_p(fpos.data_ptr()), ctypes.c_void_p(off.data_ptr()), n, _p(p),
+                      int(key) & 0xFFFFFFFFFFFFFFFF, row0, None if ids is None else ids.data_ptr(),
+                      0 if ids is None else ids.numel(), ctypes.c_void_p(out.data_ptr()), _stream_ptr(stream, d))
+            return out
         _lib.call("pss_gather", self._h, ctypes.c_void_p(data.data_ptr()), row_bytes,
                   ctypes.c_void_p(base_rows.data_ptr()), ctypes.c_void_p(fpos.data_ptr()),
                   ctypes.c_void_p(off.data_ptr()), n, ctypes.c_void_p(out.data_ptr()),

@@ -379,21 +379,36 @@ class _PartialShuffleSampler(Sampler):
             return (ids, None, None)
         return (ids,) + tuple(self._dev)
 
-    def device_batches(self, data, base_rows):
+    def dropout_key(self, site=0):
+        """The dropout key (ops.dropout, ops.combine) of this sampler's seed, current epoch and
+        logical rank at one place (`site`) of a model: with a sample's position in the rank's
+        stream as its row's id, a run resumed from state_dict() drops what the uninterrupted one
+        would have dropped, for any batch size and number of GPUs.  device_batches(p=...) uses
+        site 0."""
+        from .ops import dropout_key
+        if not self._iterated:
+            raise RuntimeError("call iter(sampler) first")
+        return dropout_key(self.seed, self._history[-1], self.rank, site)
+
+    def device_batches(self, data, base_rows, p=0.0):
         """This rank's remaining batches of the epoch gathered on the device: yields
         (rows, file_pos, offset) with rows = data[base_rows[file] + offset] for the batch's ids
         in stream order (pss_gather) -- no host round trip.  `data` holds every dataset file's
-        samples on the sampler's device, file f (dataset order) starting at row base_rows[f]."""
+        samples on the sampler's device, file f (dataset order) starting at row base_rows[f].
+        p > 0: the samples' values (float32, bfloat16 or float16) with dropout, in the same pass:
+        the mask of dropout_key(site=0) and of each sample's position in the stream."""
         if self._dev is None:
             raise RuntimeError("device_batches needs iter(sampler) first and every file length "
                                "in files_len")
         eng = self._engine
         fpos, off = self._dev
+        key = self.dropout_key() if p else 0
         while self._pos < self._end:
             lo, hi = self._pos, min(self._pos + self.batch_size, self._end)
             self._pos = hi
             self.count_batches += 1
-            yield eng.gather(data, base_rows, fpos[lo:hi], off[lo:hi]), fpos[lo:hi], off[lo:hi]
+            yield (eng.gather(data, base_rows, fpos[lo:hi], off[lo:hi], p=p, key=key, rows=lo),
+                   fpos[lo:hi], off[lo:hi])
 
     def block_indices(self):
         """[hi - lo, num_samples] ids of every logical rank of the block ranks=(lo, hi), in one
