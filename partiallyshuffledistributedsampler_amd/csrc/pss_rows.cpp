@@ -149,7 +149,7 @@ int pss_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, v
         cpu::dropout(x, ldx, residual, ldr, y, rows, cols, dtype, d, nullptr);
         return PSS_OK;
     }
-    ROWS_HIP(launch_dropout(x, ldx, residual, ldr, y, rows, cols, dtype, d, nullptr, (hipStream_t)stream));
+    ROWS_HIP(launch_dropout(x, ldx, residual, ldr, y, rows, cols, dtype, d, (hipStream_t)stream));
     return PSS_OK;
 }
 

@@ -19,13 +19,16 @@ struct Drop {
     int32_t per_row;
 };
 
-// x -> y (+ residual); strides in values.  gather: row i of x is base[order[f_i]] + off_i.
+// x -> y (+ residual); strides in values
+hipError_t launch_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows,
+                          int64_t cols, int32_t dtype, const Drop &d, hipStream_t s);
+// row i: row base[order[f_i]] + off_i of the data, f_i the file position (reflected: < 0)
 struct RowGather {
     const int64_t *base;
     const int32_t *order, *fpos, *off;
 };
-hipError_t launch_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows,
-                          int64_t cols, int32_t dtype, const Drop &d, const RowGather *g, hipStream_t s);
+hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int64_t cols, int32_t dtype, const Drop &d,
+                                 const RowGather &g, hipStream_t s);
 
 struct RouteArgs {
     const void *logits;
@@ -71,7 +74,7 @@ int make_drop(double p, uint64_t key, int64_t row0, const int64_t *ids, int64_t 
 int check_rows(const void *x, int64_t ldx, const void *y, int64_t rows, int64_t cols, int32_t dtype);
 
 namespace cpu {
-// launch_dropout on host memory
+// launch_dropout (g NULL) and launch_gather_dropout on host memory
 void dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows, int64_t cols,
              int32_t dtype, const Drop &d, const RowGather *g);
 }  // namespace cpu

@@ -26,13 +26,21 @@ template <> struct Value<_Float16> {
     static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
 };
 
+// N values as one vector of the value's alignment: one wide load or store (an array of values is taken
+// apart by the compiler and its first value's access shared with the branch for a row's end).
+template <typename T, int N> struct Pack { typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+template <typename T> struct Pack<T, 1> { typedef T V; };
+__device__ __forceinline__ float at(float v, int) { return v; }
+__device__ __forceinline__ __bf16 at(__bf16 v, int) { return v; }
+__device__ __forceinline__ _Float16 at(_Float16 v, int) { return v; }
+template <typename V> __device__ __forceinline__ auto at(const V &v, int i) { return v[i]; }
+
 template <typename T, int N>
 __device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
-    T a[N];
     if (left >= N) {
-        __builtin_memcpy(a, p, sizeof(a));
+        const typename Pack<T, N>::V a = *(const typename Pack<T, N>::V *)p;
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = Value<T>::up(a[i]);
+        for (int i = 0; i < N; i++) v[i] = Value<T>::up(at(a, i));
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = i < left ? Value<T>::up(p[i]) : 0.f;
@@ -42,10 +50,14 @@ __device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
 template <typename T, int N>
 __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
     if (left >= N) {
-        T a[N];
+        if constexpr (N == 1) {
+            *p = Value<T>::down(v[0]);
+        } else {
+            typename Pack<T, N>::V a;
 #pragma unroll
-        for (int i = 0; i < N; i++) a[i] = Value<T>::down(v[i]);
-        __builtin_memcpy(p, a, sizeof(a));
+            for (int i = 0; i < N; i++) a[i] = Value<T>::down(v[i]);
+            *(typename Pack<T, N>::V *)p = a;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -74,10 +86,10 @@ __device__ __forceinline__ void drop8(const Drop &d, int64_t r, uint32_t block, 
 }
 
 // One thread per block of 8 columns, walking over (row, block) without a division per step.
-template <typename T, bool RES, bool GATHER>
+template <typename T, bool RES>
 __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,
                                                  int64_t ldr, T *__restrict__ y, int64_t rows, int64_t cols,
-                                                 uint32_t nb, Drop d, RowGather g) {
+                                                 uint32_t nb, Drop d) {
     const int64_t step = (int64_t)gridDim.x * blockDim.x;
     const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     int64_t row = at / nb;
@@ -86,13 +98,8 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
     const uint32_t db = (uint32_t)(step - drow * nb);
     while (row < rows) {
         const int64_t c = (int64_t)b * 8, left = cols - c;
-        int64_t from = row;
-        if (GATHER) {
-            const int32_t f = g.fpos[row] < 0 ? -1 - g.fpos[row] : g.fpos[row];
-            from = g.base[g.order[f]] + g.off[row];
-        }
         float v[8];
-        load(x + from * ldx + c, left, v);
+        load(x + row * ldx + c, left, v);
         float r[8];
         if (RES) load(res + row * ldr + c, left, r);
         if (d.drop) {
@@ -434,83 +441,155 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const
     }
 }
 
-// ---- dispatch and combine ------------------------------------------------------------------------
-// A wave takes one row and a stretch of its columns, eight a lane.
-template <typename T>
-__global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restrict__ x, int64_t ldx, T *__restrict__ xs) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= m.T) return;
-    for (int64_t c = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * 8; c < m.D; c += (int64_t)gridDim.y * 512) {
-        float v[8], zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        load(x + t * ldx + c, m.D - c, v);
-        for (int j = 0; j < m.k; j++) {
-            const bool used = m.experts[t * m.k + j] >= 0;
-            store(xs + (int64_t)m.pos[t * m.k + j] * m.D + c, m.D - c, used ? v : zero);
+// ---- rows moved: gather, dispatch, combine -------------------------------------------------------
+// L lanes of a 256-thread workgroup share one row (16, 64 or all 256), eight columns a lane and step;
+// gridDim.y workgroups share its columns where there are few rows.
+template <int L>
+__device__ __forceinline__ int64_t first_row() {
+    const int sub = L >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : (int)threadIdx.x / L;
+    return (int64_t)blockIdx.x * (256 / L) + sub;
+}
+template <int L> __device__ __forceinline__ int64_t row_step() { return (int64_t)gridDim.x * (256 / L); }
+template <int L> __device__ __forceinline__ int64_t first_col() { return ((int64_t)blockIdx.y * L + threadIdx.x % L) * 8; }
+template <int L> __device__ __forceinline__ int64_t col_step() { return (int64_t)gridDim.y * L * 8; }
+
+template <typename T, int L>
+__global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data, T *__restrict__ out, int64_t rows,
+                                                     int64_t cols, Drop d, RowGather g) {
+    for (int64_t r = first_row<L>(); r < rows; r += row_step<L>()) {
+        const int32_t f = g.fpos[r] < 0 ? -1 - g.fpos[r] : g.fpos[r];
+        const T *x = data + (g.base[g.order[f]] + g.off[r]) * cols;
+        const int64_t id = drop_row(d, r);
+        for (int64_t c = first_col<L>(); c < cols; c += col_step<L>()) {
+            float v[8];
+            load(x + c, cols - c, v);
+            if (d.drop) drop8<false>(d, id, (uint32_t)(c >> 3), v, v);
+            store(out + r * cols + c, cols - c, v);
         }
     }
 }
 
-template <typename T>
+template <typename T, int L>
+__global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restrict__ x, int64_t ldx, T *__restrict__ xs) {
+    for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
+        const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
+        for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
+            float v[8];
+            const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            load(x + t * ldx + c, m.D - c, v);
+            for (int j = 0; j < m.k; j++) {
+                T *to = xs + (int64_t)pos[j] * m.D + c;
+                if (e[j] >= 0) store(to, m.D - c, v);
+                else store(to, m.D - c, zero);
+            }
+        }
+    }
+}
+
+// KU rows of y are on their way at a time.  A slot without an expert is read like any other (its place
+// is a row of y) and left out of the sum whatever it holds.
+template <typename T, int L, int KU>
 __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict__ y, const float *__restrict__ w,
                                                  const T *__restrict__ res, int64_t ldr, Drop d, T *__restrict__ out) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= m.T) return;
-    for (int64_t c = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * 8; c < m.D; c += (int64_t)gridDim.y * 512) {
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (int j = 0; j < m.k; j++) {
-            if (m.experts[t * m.k + j] < 0) continue;
-            const float wj = w ? w[t * m.k + j] : 1.f;
-            float v[8];
-            load(y + (int64_t)m.pos[t * m.k + j] * m.D + c, m.D - c, v);
+    for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
+        const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
+        const int64_t id = d.drop ? drop_row(d, t) : 0;
+        for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
+            float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (res) load(res + t * ldr + c, m.D - c, r);
+            for (int j0 = 0; j0 < m.k; j0 += KU) {
+                float v[KU][8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[i] = fmaf(wj, v[i], acc[i]);
-        }
-        float r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (res) load(res + t * ldr + c, m.D - c, r);
-        if (d.drop) {
-            drop8<true>(d, drop_row(d, t), (uint32_t)(c >> 3), acc, r);
-        } else if (res) {
+                for (int u = 0; u < KU; u++) {
+                    const int j = j0 + u < m.k ? j0 + u : j0;
+                    load(y + (int64_t)pos[j] * m.D + c, m.D - c, v[u]);
+                }
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[i] += r[i];
+                for (int u = 0; u < KU; u++) {
+                    const int j = j0 + u < m.k ? j0 + u : j0;
+                    const bool on = j0 + u < m.k && e[j] >= 0;
+                    const float wj = w ? w[t * m.k + j] : 1.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) acc[i] = on ? fmaf(wj, v[u][i], acc[i]) : acc[i];
+                }
+            }
+            if (d.drop) {
+                drop8<true>(d, id, (uint32_t)(c >> 3), acc, r);
+            } else if (res) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[i] += r[i];
+            }
+            store(out + t * m.D + c, m.D - c, acc);
         }
-        store(out + t * m.D + c, m.D - c, acc);
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const T *__restrict__ dout, int64_t ldo,
+// One pass over g = dropout(dout): KU products with rows of y and KU rows of dy at a time.  The lanes
+// of a row hold partial products of all its slots; they are joined after the last column.
+template <typename T, int L, int KM>
+__global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t *__restrict__ experts,
+                                                      const int32_t *__restrict__ places, const T *__restrict__ dout, int64_t ldo,
                                                       const T *__restrict__ y, const float *__restrict__ w, Drop d,
                                                       T *__restrict__ dy, float *__restrict__ dw) {
-    const int64_t t = blockIdx.x;
-    __shared__ float part[4];
-    for (int j = 0; j < m.k; j++) {
-        const int64_t slot = t * m.k + j;
-        const bool used = m.experts[slot] >= 0;
-        const int64_t p = m.pos[slot];
-        const float wj = used ? w[slot] : 0.f;
-        float dot = 0.f;
-        for (int64_t c = (int64_t)threadIdx.x * 8; c < m.D; c += 256 * 8) {
-            float g[8], o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (used) {
-                load(dout + t * ldo + c, m.D - c, g);
-                if (d.drop) drop8<false>(d, drop_row(d, t), (uint32_t)(c >> 3), g, g);
+    constexpr int KU = KM < 8 ? KM : 8;
+    __shared__ float part[L > 64 ? 4 : 1][KM];
+    for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
+        const int64_t id = d.drop ? drop_row(d, t) : 0;
+        float dot[KM], wt[KM];
+        int32_t pos[KM];
+        bool on[KM];
+#pragma unroll
+        for (int j = 0; j < KM; j++) {
+            const int64_t slot = t * m.k + (j < m.k ? j : 0);
+            on[j] = experts[slot] >= 0;
+            pos[j] = places[slot];
+            wt[j] = w[slot];
+            dot[j] = 0.f;
+        }
+        for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
+            float g[8];
+            load(dout + t * ldo + c, m.D - c, g);
+            if (d.drop) drop8<false>(d, id, (uint32_t)(c >> 3), g, g);
+#pragma unroll
+            for (int j0 = 0; j0 < KM; j0 += KU) {
+                if (j0 >= m.k) break;
                 if (dw) {
-                    float v[8];
-                    load(y + p * m.D + c, m.D - c, v);
+                    float v[KU][8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) dot = fmaf(g[i], v[i], dot);
+                    for (int u = 0; u < KU; u++) load(y + (int64_t)pos[j0 + u] * m.D + c, m.D - c, v[u]);
+#pragma unroll
+                    for (int u = 0; u < KU; u++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) dot[j0 + u] = fmaf(g[i], v[u][i], dot[j0 + u]);
                 }
+                if (dy) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[i] = wj * g[i];
+                    for (int u = 0; u < KU; u++) {
+                        if (j0 + u >= m.k) break;
+                        float o[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] = on[j0 + u] ? wt[j0 + u] * g[i] : 0.f;
+                        store(dy + (int64_t)pos[j0 + u] * m.D + c, m.D - c, o);
+                    }
+                }
             }
-            if (dy) store(dy + p * m.D + c, m.D - c, o);
         }
         if (!dw) continue;
-        dot = seg_reduce<64>(dot, [](float a, float b) { return a + b; });
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) dw[slot] = part[0] + part[1] + part[2] + part[3];
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < KM; j++) dot[j] = seg_reduce<(L < 64 ? L : 64)>(dot[j], [](float a, float b) { return a + b; });
+        if (L > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int j = 0; j < KM; j++) part[threadIdx.x >> 6][j] = dot[j];
+            __syncthreads();
+            const int j = threadIdx.x;
+            if (j < m.k) dw[t * m.k + j] = experts[t * m.k + j] >= 0 ? (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]) : 0.f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < KM; j++)
+                if ((threadIdx.x & (L - 1)) == (j & (L - 1)) && j < m.k) dw[t * m.k + j] = on[j] ? dot[j] : 0.f;
+        }
     }
 }
 
@@ -539,24 +618,57 @@ void by_width(int E, F f) {
 
 }  // namespace
 
+// lanes of a row of `cols` values, and the launch of `rows` such rows
+template <typename F>
+static void by_row(int64_t rows, int64_t cols, F f) {
+    const int L = cols <= 128 ? 16 : cols <= 1024 ? 64 : 256;
+    int64_t x = (rows + 256 / L - 1) / (256 / L), y = 1;
+    if (x < 2048) {      // few rows: their columns over several workgroups
+        y = (cols + L * 8 - 1) / (L * 8);
+        if (y > 2048 / x) y = 2048 / x;
+        if (y < 1) y = 1;
+    }
+    const dim3 grid((unsigned)(x < (1 << 20) ? x : 1 << 20), (unsigned)y);
+    if (L == 16) f(std::integral_constant<int, 16>(), grid);
+    else if (L == 64) f(std::integral_constant<int, 64>(), grid);
+    else f(std::integral_constant<int, 256>(), grid);
+}
+
+template <typename F>
+static void by_slots(int k, F f) {
+    if (k <= 1) f(std::integral_constant<int, 1>());
+    else if (k <= 2) f(std::integral_constant<int, 2>());
+    else if (k <= 4) f(std::integral_constant<int, 4>());
+    else if (k <= 8) f(std::integral_constant<int, 8>());
+    else f(std::integral_constant<int, 16>());
+}
+
 hipError_t launch_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows,
-                          int64_t cols, int32_t dtype, const Drop &d, const RowGather *g, hipStream_t s) {
+                          int64_t cols, int32_t dtype, const Drop &d, hipStream_t s) {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const int64_t nb = (cols + 7) / 8, n = rows * nb;
     const int64_t blocks = (n + 255) / 256;
     const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-    const RowGather gg = g ? *g : RowGather{};
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        if (g)
-            hipLaunchKernelGGL((k_dropout<T, false, true>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)nullptr,
-                               (int64_t)0, (T *)y, rows, cols, (uint32_t)nb, d, gg);
-        else if (residual)
-            hipLaunchKernelGGL((k_dropout<T, true, false>), grid, dim3(256), 0, s, (const T *)x, ldx,
-                               (const T *)residual, ldr, (T *)y, rows, cols, (uint32_t)nb, d, gg);
+        if (residual)
+            hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)residual, ldr,
+                               (T *)y, rows, cols, (uint32_t)nb, d);
         else
-            hipLaunchKernelGGL((k_dropout<T, false, false>), grid, dim3(256), 0, s, (const T *)x, ldx,
-                               (const T *)nullptr, (int64_t)0, (T *)y, rows, cols, (uint32_t)nb, d, gg);
+            hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)nullptr,
+                               (int64_t)0, (T *)y, rows, cols, (uint32_t)nb, d);
+    });
+}
+
+hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int64_t cols, int32_t dtype, const Drop &d,
+                                 const RowGather &g, hipStream_t s) {
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    return by_type(dtype, [&](auto *p) {
+        using T = std::remove_pointer_t<decltype(p)>;
+        by_row(rows, cols, [&](auto L, dim3 grid) {
+            hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value>), grid, dim3(256), 0, s, (const T *)data, (T *)out,
+                               rows, cols, d, g);
+        });
     });
 }
 
@@ -594,16 +706,13 @@ hipError_t launch_route_grad(const RouteArgs &a, const float *dweights, void *dl
     });
 }
 
-static dim3 move_grid(const MoveArgs &m) {
-    const int64_t cols = (m.D + 511) / 512;
-    return dim3((unsigned)((m.T + 3) / 4), (unsigned)(cols < 64 ? cols : 64));
-}
-
 hipError_t launch_dispatch(const MoveArgs &m, const void *x, int64_t ldx, void *xs, hipStream_t s) {
     if (m.T <= 0 || m.D <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        hipLaunchKernelGGL(k_dispatch<T>, move_grid(m), dim3(256), 0, s, m, (const T *)x, ldx, (T *)xs);
+        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+            hipLaunchKernelGGL((k_dispatch<T, decltype(L)::value>), grid, dim3(256), 0, s, m, (const T *)x, ldx, (T *)xs);
+        });
     });
 }
 
@@ -612,8 +721,12 @@ hipError_t launch_combine(const MoveArgs &m, const void *y, const float *w, cons
     if (m.T <= 0 || m.D <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        hipLaunchKernelGGL(k_combine<T>, move_grid(m), dim3(256), 0, s, m, (const T *)y, w, (const T *)residual, ldr,
-                           d, (T *)out);
+        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+            by_slots(m.k < 8 ? m.k : 8, [&](auto KU) {
+                hipLaunchKernelGGL((k_combine<T, decltype(L)::value, decltype(KU)::value>), grid, dim3(256), 0, s, m,
+                                   (const T *)y, w, (const T *)residual, ldr, d, (T *)out);
+            });
+        });
     });
 }
 
@@ -622,8 +735,13 @@ hipError_t launch_combine_grad(const MoveArgs &m, const void *dout, int64_t ldo,
     if (m.T <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        hipLaunchKernelGGL(k_combine_grad<T>, dim3((unsigned)m.T), dim3(256), 0, s, m, (const T *)dout, ldo,
-                           (const T *)y, w, d, (T *)dy, dw);
+        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+            grid.y = 1;     // the products run over all columns
+            by_slots(m.k, [&](auto KM) {
+                hipLaunchKernelGGL((k_combine_grad<T, decltype(L)::value, decltype(KM)::value>), grid, dim3(256), 0, s,
+                                   m, m.experts, m.pos, (const T *)dout, ldo, (const T *)y, w, d, (T *)dy, dw);
+            });
+        });
     });
 }
 

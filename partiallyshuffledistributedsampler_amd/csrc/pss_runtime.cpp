@@ -1417,7 +1417,7 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
     rc = prepare_tables(h, s);
     if (rc) return rc;
     const pss::RowGather g{base_rows_dev, h->tab[h->tab_cur].order, file_pos_dev, offset_dev};
-    PSS_HIP(pss::launch_dropout(data_dev, row_values, nullptr, 0, out_dev, n, row_values, dtype, d, &g, s));
+    PSS_HIP(pss::launch_gather_dropout(data_dev, out_dev, n, row_values, dtype, d, g, s));
     return tables_read(h, s);
 }
 

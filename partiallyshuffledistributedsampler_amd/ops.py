@@ -58,24 +58,28 @@ def dropout_key(seed, epoch, rank=0, site=0):
 
 
 # ---- plumbing ------------------------------------------------------------------------------------
-class _on:
-    """The tensors' device as the current one (nothing to do where it already is)."""
-
-    def __init__(self, device):
-        i = device.index
-        self.guard = None if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name, device, *args):
+    """The C entry with the current stream of `device` (which it makes the current one) as the last
+    argument."""
+    fn = getattr(_lib.load(), name)
+    i = device.index
+    if i != torch.cuda.current_device():
+        with torch.cuda.device(i):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _stream(device):
-    return 0 if device.type == "cpu" else torch.cuda.current_stream(device).cuda_stream
+def _once(backward):
+    """A backward pass that cannot be differentiated itself: torch's once_differentiable where a
+    graph of it is asked for, the plain function (without its overhead) where not."""
+    wrapped = once_differentiable(backward)
+
+    def f(ctx, *grads):
+        return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(f)
 
 
 def _ptr(t):
@@ -134,13 +138,11 @@ def _dropout(x, residual, p, key, row0, ids):
     ldr = 0
     if residual is not None:
         residual, _, _, ldr = _rows2d(residual)
+    args = (x2.data_ptr(), ld, _ptr(residual), ldr, y.data_ptr(), n, d, DTYPES[x.dtype], p, key, row0, _ptr(ids), _n(ids))
     if x.device.type == "cpu":
-        _lib.call("pss_dropout", x2.data_ptr(), ld, _ptr(residual), ldr, y.data_ptr(), n, d, DTYPES[x.dtype], p, key,
-                  row0, _ptr(ids), _n(ids), 1, None)
+        _lib.call("pss_dropout", *args, 1, None)
     else:
-        with _on(x.device):
-            _lib.call("pss_dropout", x2.data_ptr(), ld, _ptr(residual), ldr, y.data_ptr(), n, d, DTYPES[x.dtype], p,
-                      key, row0, _ptr(ids), _n(ids), 0, _stream(x.device))
+        _call("pss_dropout", x.device, *args, 0)
     return y
 
 
@@ -151,8 +153,7 @@ class _Dropout(torch.autograd.Function):
         ctx.save_for_backward(ids)
         return _dropout(x, residual, p, key, row0, ids)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         p, key, row0 = ctx.args
         dx = _dropout(dy, None, p, key, row0, *ctx.saved_tensors) if ctx.needs_input_grad[0] else None
@@ -194,10 +195,9 @@ def _route(logits, k, score, bias, valid, groups, top_groups, group_sum, renorma
     src = torch.empty(n * k, dtype=i32, device=dev)
     need = _lib.load().pss_route_workspace(n, e)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        _lib.call("pss_route", l2.data_ptr(), ld, n, e, k, DTYPES[logits.dtype], score, _ptr(bias), _ptr(valid), groups,
-                  top_groups, group_sum, renormalise, scale, experts.data_ptr(), weights.data_ptr(),
-                  offsets.data_ptr(), pos.data_ptr(), src.data_ptr(), _ptr(ws), need, _stream(dev))
+    _call("pss_route", dev, l2.data_ptr(), ld, n, e, k, DTYPES[logits.dtype], score, _ptr(bias), _ptr(valid), groups,
+          top_groups, group_sum, renormalise, scale, experts.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
+          pos.data_ptr(), src.data_ptr(), _ptr(ws), need)
     return experts, weights, offsets, pos, src
 
 
@@ -211,8 +211,7 @@ class _Route(torch.autograd.Function):
         ctx.args = k, score, renormalise, scale
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, _experts, dweights, *_plan):
         if dweights is None or not ctx.needs_input_grad[0]:
             return (None,) * 10
@@ -221,10 +220,8 @@ class _Route(torch.autograd.Function):
         l2, n, e, ld = _rows2d(logits)
         dweights = dweights.contiguous()
         dlogits = torch.empty((n, e), dtype=logits.dtype, device=logits.device)
-        with _on(logits.device):
-            _lib.call("pss_route_grad", l2.data_ptr(), ld, n, e, k, DTYPES[logits.dtype], score, renormalise, scale,
-                      experts.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(),
-                      _stream(logits.device))
+        _call("pss_route_grad", logits.device, l2.data_ptr(), ld, n, e, k, DTYPES[logits.dtype], score, renormalise,
+              scale, experts.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
         return (dlogits,) + (None,) * 9
 
 
@@ -287,9 +284,8 @@ def _dispatch(x, experts, pos):
     x2, n, d, ld = _rows2d(x)
     k = pos.shape[1]
     xs = torch.empty((n * k, d), dtype=x.dtype, device=x.device)
-    with _on(x.device):
-        _lib.call("pss_dispatch", x2.data_ptr(), ld, n, k, d, DTYPES[x.dtype], experts.data_ptr(), pos.data_ptr(),
-                  xs.data_ptr(), _stream(x.device))
+    _call("pss_dispatch", x.device, x2.data_ptr(), ld, n, k, d, DTYPES[x.dtype], experts.data_ptr(), pos.data_ptr(),
+          xs.data_ptr())
     return xs
 
 
@@ -301,10 +297,8 @@ def _combine(y, experts, pos, weights, residual, p, key, row0, ids):
     ldr = 0
     if residual is not None:
         residual, _, _, ldr = _rows2d(residual)
-    with _on(y.device):
-        _lib.call("pss_combine", y.data_ptr(), n, k, d, DTYPES[y.dtype], experts.data_ptr(), pos.data_ptr(),
-                  _ptr(weights), _ptr(residual), ldr, p, key, row0, _ptr(ids), _n(ids), out.data_ptr(),
-                  _stream(y.device))
+    _call("pss_combine", y.device, y.data_ptr(), n, k, d, DTYPES[y.dtype], experts.data_ptr(), pos.data_ptr(),
+          _ptr(weights), _ptr(residual), ldr, p, key, row0, _ptr(ids), _n(ids), out.data_ptr())
     return out
 
 
@@ -314,8 +308,7 @@ class _Dispatch(torch.autograd.Function):
         ctx.save_for_backward(experts, pos)
         return _dispatch(x, experts, pos)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dxs):
         experts, pos = ctx.saved_tensors
         return _combine(dxs, experts, pos, None, None, 0.0, 0, 0, None), None, None
@@ -328,8 +321,7 @@ class _Combine(torch.autograd.Function):
         ctx.args = p, key, row0
         return _combine(y, experts, pos, weights, residual, p, key, row0, ids)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         want_y, want_w, want_r = ctx.needs_input_grad[:3]
         dy = dw = None
@@ -341,10 +333,9 @@ class _Combine(torch.autograd.Function):
             d2, _, d, ld = _rows2d(dout)
             dy = torch.empty_like(y) if want_y else None
             dw = torch.empty((n, k), dtype=torch.float32, device=y.device) if want_w else None
-            with _on(y.device):
-                _lib.call("pss_combine_grad", d2.data_ptr(), ld, y.data_ptr(), n, k, d, DTYPES[y.dtype],
-                          experts.data_ptr(), pos.data_ptr(), weights.data_ptr(), p, key, row0, _ptr(ids), _n(ids),
-                          _ptr(dy), _ptr(dw), _stream(y.device))
+            _call("pss_combine_grad", y.device, d2.data_ptr(), ld, y.data_ptr(), n, k, d, DTYPES[y.dtype],
+                  experts.data_ptr(), pos.data_ptr(), weights.data_ptr(), p, key, row0, _ptr(ids), _n(ids), _ptr(dy),
+                  _ptr(dw))
         return (dy, dw, dout if want_r else None) + (None,) * 6
 
 
