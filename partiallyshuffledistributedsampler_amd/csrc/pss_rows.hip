@@ -35,10 +35,12 @@ __device__ __forceinline__ __bf16 at(__bf16 v, int) { return v; }
 __device__ __forceinline__ _Float16 at(_Float16 v, int) { return v; }
 template <typename V> __device__ __forceinline__ auto at(const V &v, int i) { return v[i]; }
 
-template <typename T, int N>
+// NT: past the caches (nontemporal)
+template <bool NT = false, typename T, int N>
 __device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
     if (left >= N) {
-        const typename Pack<T, N>::V a = *(const typename Pack<T, N>::V *)p;
+        typedef typename Pack<T, N>::V V;
+        const V a = NT ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = Value<T>::up(at(a, i));
     } else {
@@ -47,7 +49,7 @@ __device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
     }
 }
 
-template <typename T, int N>
+template <bool NT = false, typename T, int N>
 __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
     if (left >= N) {
         if constexpr (N == 1) {
@@ -56,7 +58,8 @@ __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
             typename Pack<T, N>::V a;
 #pragma unroll
             for (int i = 0; i < N; i++) a[i] = Value<T>::down(v[i]);
-            *(typename Pack<T, N>::V *)p = a;
+            if (NT) __builtin_nontemporal_store(a, (typename Pack<T, N>::V *)p);
+            else *(typename Pack<T, N>::V *)p = a;
         }
     } else {
 #pragma unroll
@@ -71,22 +74,27 @@ __device__ __forceinline__ int64_t drop_row(const Drop &d, int64_t i) {
     return d.row0 + (d.per_row ? d.ids[i] : d.ids[0] + i);
 }
 
-// Eight values of a row with id r from column 8 * block on: v * scale (+ add, in one rounding as the
-// CPU mode's fma) where kept; an exact 0 (add) where not, also of an infinity or a NaN.
-template <bool ADD>
-__device__ __forceinline__ void drop8(const Drop &d, int64_t r, uint32_t block, float (&v)[8], const float (&add)[8]) {
+// The eight draws of a block of columns of the row with id r.
+struct Draw { uint32_t w[4]; };
+__device__ __forceinline__ Draw draw8(const Drop &d, int64_t r, uint32_t block) {
     uint32_t c0 = block, c1 = (uint32_t)r, c2 = (uint32_t)((uint64_t)r >> 32), c3 = DOM_DROPOUT;
     philox4x32_10(c0, c1, c2, c3, d.key0, d.key1);
-    const uint32_t w[4] = {c0, c1, c2, c3};
+    return Draw{{c0, c1, c2, c3}};
+}
+
+// v * scale (+ add, in one rounding as the CPU mode's fma) where kept; an exact 0 (add) where not,
+// also of an infinity or a NaN.
+template <bool ADD>
+__device__ __forceinline__ void drop8(const Drop &d, const Draw &u, float (&v)[8], const float (&add)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t u = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu;
-        v[i] = u >= d.drop ? (ADD ? fmaf(v[i], d.scale, add[i]) : v[i] * d.scale) : (ADD ? add[i] : 0.f);
+        const uint32_t x = (i & 1) ? u.w[i >> 1] >> 16 : u.w[i >> 1] & 0xFFFFu;
+        v[i] = x >= d.drop ? (ADD ? fmaf(v[i], d.scale, add[i]) : v[i] * d.scale) : (ADD ? add[i] : 0.f);
     }
 }
 
 // One thread per block of 8 columns, walking over (row, block) without a division per step.
-template <typename T, bool RES>
+template <typename T, bool RES, bool NT>
 __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,
                                                  int64_t ldr, T *__restrict__ y, int64_t rows, int64_t cols,
                                                  uint32_t nb, Drop d) {
@@ -99,16 +107,16 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
     while (row < rows) {
         const int64_t c = (int64_t)b * 8, left = cols - c;
         float v[8];
-        load(x + row * ldx + c, left, v);
+        load<NT>(x + row * ldx + c, left, v);
         float r[8];
-        if (RES) load(res + row * ldr + c, left, r);
+        if (RES) load<NT>(res + row * ldr + c, left, r);
         if (d.drop) {
-            drop8<RES>(d, drop_row(d, row), b, v, r);
+            drop8<RES>(d, draw8(d, drop_row(d, row), b), v, r);
         } else if (RES) {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] += r[i];
         }
-        store(y + row * cols + c, left, v);
+        store<NT>(y + row * cols + c, left, v);
         row += drow;
         b += db;
         if (b >= nb) { b -= nb; row++; }
@@ -453,7 +461,7 @@ template <int L> __device__ __forceinline__ int64_t row_step() { return (int64_t
 template <int L> __device__ __forceinline__ int64_t first_col() { return ((int64_t)blockIdx.y * L + threadIdx.x % L) * 8; }
 template <int L> __device__ __forceinline__ int64_t col_step() { return (int64_t)gridDim.y * L * 8; }
 
-template <typename T, int L>
+template <typename T, int L, bool NT>
 __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data, T *__restrict__ out, int64_t rows,
                                                      int64_t cols, Drop d, RowGather g) {
     for (int64_t r = first_row<L>(); r < rows; r += row_step<L>()) {
@@ -462,9 +470,9 @@ __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data,
         const int64_t id = drop_row(d, r);
         for (int64_t c = first_col<L>(); c < cols; c += col_step<L>()) {
             float v[8];
-            load(x + c, cols - c, v);
-            if (d.drop) drop8<false>(d, id, (uint32_t)(c >> 3), v, v);
-            store(out + r * cols + c, cols - c, v);
+            load<NT>(x + c, cols - c, v);
+            if (d.drop) drop8<false>(d, draw8(d, id, (uint32_t)(c >> 3)), v, v);
+            store<NT>(out + r * cols + c, cols - c, v);
         }
     }
 }
@@ -488,7 +496,7 @@ __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restric
 
 // KU rows of y are on their way at a time.  A slot without an expert is read like any other (its place
 // is a row of y) and left out of the sum whatever it holds.
-template <typename T, int L, int KU>
+template <typename T, int L, int KU, bool NT>
 __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict__ y, const float *__restrict__ w,
                                                  const T *__restrict__ res, int64_t ldr, Drop d, T *__restrict__ out) {
     for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
@@ -496,14 +504,16 @@ __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict
         const int64_t id = d.drop ? drop_row(d, t) : 0;
         for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
             float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (res) load(res + t * ldr + c, m.D - c, r);
+            if (res) load<NT>(res + t * ldr + c, m.D - c, r);
+            Draw dr;
             for (int j0 = 0; j0 < m.k; j0 += KU) {
                 float v[KU][8];
 #pragma unroll
                 for (int u = 0; u < KU; u++) {
                     const int j = j0 + u < m.k ? j0 + u : j0;
-                    load(y + (int64_t)pos[j] * m.D + c, m.D - c, v[u]);
+                    load<NT>(y + (int64_t)pos[j] * m.D + c, m.D - c, v[u]);
                 }
+                if (d.drop && j0 == 0) dr = draw8(d, id, (uint32_t)(c >> 3));   // while the rows come
 #pragma unroll
                 for (int u = 0; u < KU; u++) {
                     const int j = j0 + u < m.k ? j0 + u : j0;
@@ -514,12 +524,12 @@ __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict
                 }
             }
             if (d.drop) {
-                drop8<true>(d, id, (uint32_t)(c >> 3), acc, r);
+                drop8<true>(d, dr, acc, r);
             } else if (res) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) acc[i] += r[i];
             }
-            store(out + t * m.D + c, m.D - c, acc);
+            store<NT>(out + t * m.D + c, m.D - c, acc);
         }
     }
 }
@@ -549,7 +559,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
         for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
             float g[8];
             load(dout + t * ldo + c, m.D - c, g);
-            if (d.drop) drop8<false>(d, id, (uint32_t)(c >> 3), g, g);
+            if (d.drop) drop8<false>(d, draw8(d, id, (uint32_t)(c >> 3)), g, g);
 #pragma unroll
             for (int j0 = 0; j0 < KM; j0 += KU) {
                 if (j0 >= m.k) break;
@@ -618,6 +628,19 @@ void by_width(int E, F f) {
 
 }  // namespace
 
+// Whether a pass over so many bytes goes past the caches: beyond the 256 MB of the Infinity Cache
+// nothing of it can be found there later.  Measured past / through: dropout 16384 x 8192 bf16 with
+// residual 131 / 157 us, without 91 / 94; gather of 65536 x 2048 bf16 99 / 125; combine of
+// 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16 (17 MB) 7.8 / 7.4.  Dispatch and
+// the combine's gradient write eight rows for one read and are slower past them (249 / 223, 474 / 458).
+static bool past_caches(int64_t bytes) { return bytes > ((int64_t)256 << 20); }
+
+template <typename F>
+static void by_flag(bool b, F f) {
+    if (b) f(std::true_type());
+    else f(std::false_type());
+}
+
 // lanes of a row of `cols` values, and the launch of `rows` such rows
 template <typename F>
 static void by_row(int64_t rows, int64_t cols, F f) {
@@ -651,12 +674,12 @@ hipError_t launch_dropout(const void *x, int64_t ldx, const void *residual, int6
     const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        if (residual)
-            hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)residual, ldr,
-                               (T *)y, rows, cols, (uint32_t)nb, d);
-        else
-            hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)nullptr,
-                               (int64_t)0, (T *)y, rows, cols, (uint32_t)nb, d);
+        by_flag(past_caches(rows * cols * (int64_t)sizeof(T) * (residual ? 3 : 2)), [&](auto NT) {
+            by_flag(residual != nullptr, [&](auto RES) {
+                hipLaunchKernelGGL((k_dropout<T, decltype(RES)::value, decltype(NT)::value>), grid, dim3(256), 0, s,
+                                   (const T *)x, ldx, (const T *)residual, ldr, (T *)y, rows, cols, (uint32_t)nb, d);
+            });
+        });
     });
 }
 
@@ -666,8 +689,10 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
         by_row(rows, cols, [&](auto L, dim3 grid) {
-            hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value>), grid, dim3(256), 0, s, (const T *)data, (T *)out,
-                               rows, cols, d, g);
+            by_flag(past_caches(2 * rows * cols * (int64_t)sizeof(T)), [&](auto NT) {
+                hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value, decltype(NT)::value>), grid, dim3(256), 0, s,
+                                   (const T *)data, (T *)out, rows, cols, d, g);
+            });
         });
     });
 }
@@ -723,8 +748,10 @@ hipError_t launch_combine(const MoveArgs &m, const void *y, const float *w, cons
         using T = std::remove_pointer_t<decltype(p)>;
         by_row(m.T, m.D, [&](auto L, dim3 grid) {
             by_slots(m.k < 8 ? m.k : 8, [&](auto KU) {
-                hipLaunchKernelGGL((k_combine<T, decltype(L)::value, decltype(KU)::value>), grid, dim3(256), 0, s, m,
-                                   (const T *)y, w, (const T *)residual, ldr, d, (T *)out);
+                by_flag(past_caches(m.T * (m.k + 2) * m.D * (int64_t)sizeof(T)), [&](auto NT) {
+                    hipLaunchKernelGGL((k_combine<T, decltype(L)::value, decltype(KU)::value, decltype(NT)::value>), grid,
+                                       dim3(256), 0, s, m, (const T *)y, w, (const T *)residual, ldr, d, (T *)out);
+                });
             });
         });
     });
