@@ -181,7 +181,7 @@ static int route_args(RouteArgs *a, const void *logits, int64_t ld, int64_t toke
 int64_t pss_route_workspace(int64_t tokens, int32_t experts) {
     if (tokens < 0 || experts < 1) return 0;
     const int64_t n = route_chunks(tokens);
-    return n > 1 ? n * experts * (int64_t)sizeof(uint16_t) : 0;
+    return n > 1 ? (n * 12 + 4) * experts : 0;
 }
 
 int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype, int32_t score,
@@ -200,7 +200,8 @@ int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, i
     if (!offsets || (tokens > 0 && (!out_experts || !out_weights || !pos || !src)))
         return set_error(PSS_EINVAL, "route: NULL output");
     const int64_t need = pss_route_workspace(tokens, experts);
-    if (need > 0 && (!ws || ws_bytes < need)) return set_error(PSS_EINVAL, "route: the workspace is too small");
+    if (need > 0 && (!ws || ws_bytes < need || (uintptr_t)ws % 8))
+        return set_error(PSS_EINVAL, "route: the workspace is too small, or not 8-byte aligned");
     a.bias = bias;
     a.valid = valid;
     a.groups = groups;
@@ -211,7 +212,12 @@ int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, i
     a.offsets = offsets;
     a.pos = pos;
     a.src = src;
-    a.hist = need > 0 ? (uint16_t *)ws : nullptr;
+    if (need > 0) {
+        const int64_t n = route_chunks(tokens) * experts;
+        a.mask = (uint64_t *)ws;
+        a.before = (int32_t *)(a.mask + n);
+        a.totals = a.before + n;
+    }
     ROWS_HIP(launch_route(a, (hipStream_t)stream));
     return PSS_OK;
 }

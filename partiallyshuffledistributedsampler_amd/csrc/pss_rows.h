@@ -45,9 +45,12 @@ struct RouteArgs {
     float *weights;         // [T, k]
     int32_t *offsets;       // [E + 1]
     int32_t *pos, *src;     // [T * k]
-    uint16_t *hist;         // [chunks, E]; NULL with one chunk
+    // workspace (NULL with one chunk): rows of each chunk and expert, rows before, rows in all
+    uint64_t *mask;         // [chunks, E]
+    int32_t *before;        // [chunks, E]
+    int32_t *totals;        // [E]
 };
-constexpr int kRouteChunk = 256;    // rows whose places one workgroup assigns
+constexpr int kRouteChunk = 64;     // rows of a workgroup: one bit of a 64-bit mask each
 constexpr int kRouteMaxE = 1024, kRouteMaxK = 16, kRouteMaxGroups = 64;
 static inline int64_t route_chunks(int64_t T) { return T <= kRouteChunk ? 1 : (T + kRouteChunk - 1) / kRouteChunk; }
 hipError_t launch_route(const RouteArgs &a, hipStream_t s);

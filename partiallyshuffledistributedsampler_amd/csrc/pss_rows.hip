@@ -2,6 +2,8 @@
 // row ids, routing to experts, dispatch into expert order and combination by weight (pss_rows.h).
 #include <math.h>
 
+#include <algorithm>
+
 #include "pss_common.h"
 #include "pss_device.h"
 #include "pss_rows.h"
@@ -37,7 +39,7 @@ template <typename V> __device__ __forceinline__ auto at(const V &v, int i) { re
 
 // NT: past the caches (nontemporal)
 template <bool NT = false, typename T, int N>
-__device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
+__device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N], float fill = 0.f) {
     if (left >= N) {
         typedef typename Pack<T, N>::V V;
         const V a = NT ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
@@ -45,7 +47,7 @@ __device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
         for (int i = 0; i < N; i++) v[i] = Value<T>::up(at(a, i));
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < left ? Value<T>::up(p[i]) : 0.f;
+        for (int i = 0; i < N; i++) v[i] = i < left ? Value<T>::up(p[i]) : fill;
     }
 }
 
@@ -124,12 +126,56 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
 }
 
 // ---- routing -------------------------------------------------------------------------------------
-// The lanes of a segment (16 or 64 of a wave) share one row; reductions stay inside the segment.
+// The lanes of a segment (16 or 64 of a wave) share one row; reductions stay inside the segment.  Step
+// i joins lanes that hold the same after the steps before: 1 and 2 apart, then the halves of 8 and 16
+// mirrored (DPP, no LDS), then 16 and 32 apart.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_mov(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, true);
+}
+template <int I> __device__ __forceinline__ uint32_t partner32(uint32_t x) {
+    if constexpr (I == 0) return dpp_mov<0xB1>(x);
+    else if constexpr (I == 1) return dpp_mov<0x4E>(x);
+    else if constexpr (I == 2) return dpp_mov<0x141>(x);
+    else if constexpr (I == 3) return dpp_mov<0x140>(x);
+    else return (uint32_t)__shfl_xor((int)x, 1 << I, 64);
+}
+template <int I, typename T> __device__ __forceinline__ T partner(T x) {
+    if constexpr (sizeof(T) == 4) {
+        uint32_t u;
+        __builtin_memcpy(&u, &x, 4);
+        u = partner32<I>(u);
+        __builtin_memcpy(&x, &u, 4);
+    } else {
+        static_assert(sizeof(T) == 8);
+        uint32_t u[2];
+        __builtin_memcpy(u, &x, 8);
+        u[0] = partner32<I>(u[0]);
+        u[1] = partner32<I>(u[1]);
+        __builtin_memcpy(&x, u, 8);
+    }
+    return x;
+}
 template <int L, typename T, typename F>
 __device__ __forceinline__ T seg_reduce(T v, F f) {
-#pragma unroll
-    for (int m = L / 2; m; m >>= 1) v = f(v, __shfl_xor(v, m, 64));
+    v = f(v, partner<0>(v));
+    v = f(v, partner<1>(v));
+    v = f(v, partner<2>(v));
+    v = f(v, partner<3>(v));
+    if constexpr (L == 64) {
+        v = f(v, partner<4>(v));
+        v = f(v, partner<5>(v));
+    }
     return v;
+}
+struct Max { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
+struct Min { template <typename T> __device__ T operator()(T a, T b) const { return a < b ? a : b; } };
+struct Sum { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
+struct Or { template <typename T> __device__ T operator()(T a, T b) const { return a | b; } };
+template <int L> __device__ __forceinline__ float seg_max(float v) {
+    return seg_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int L> __device__ __forceinline__ float seg_min(float v) {
+    return seg_reduce<L>(v, [](float a, float b) { return fminf(a, b); });
 }
 
 __device__ __forceinline__ void wave_lds_sync() {
@@ -138,41 +184,171 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// N logits of row t from expert e0 on, -inf past the last
+template <int N>
+__device__ __forceinline__ void load_logits(const RouteArgs &a, int64_t t, int e0, float (&l)[N]) {
+    const int64_t i = t * a.ld + e0;
+    if (a.dtype == 0) load((const float *)a.logits + i, a.E - e0, l, -INFINITY);
+    else if (a.dtype == 1) load((const __bf16 *)a.logits + i, a.E - e0, l, -INFINITY);
+    else load((const _Float16 *)a.logits + i, a.E - e0, l, -INFINITY);
+}
+__device__ __forceinline__ float one_logit(const RouteArgs &a, int64_t t, int e) {
+    const int64_t i = t * a.ld + e;
+    if (a.dtype == 0) return ((const float *)a.logits)[i];
+    if (a.dtype == 1) return (float)((const __bf16 *)a.logits)[i];
+    return (float)((const _Float16 *)a.logits)[i];
+}
+
+// exp of a difference of logits (<= 0): off by 2^-24 of the exponent and one unit of the result
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// Sorted lists (falling) of unsigned keys, in registers.
+__device__ __forceinline__ void order2(uint32_t &a, uint32_t &b) {
+    const uint32_t hi = a > b ? a : b, lo = a > b ? b : a;
+    a = hi;
+    b = lo;
+}
+template <int N> __device__ __forceinline__ void bitonic(uint32_t *x) {   // a bitonic list into falling order
+#pragma unroll
+    for (int h = N / 2; h; h >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (!(i & h)) order2(x[i], x[i + h]);
+}
+// x[0, N) any -> falling (bitonic network)
+template <int N> __device__ __forceinline__ void sort_falling(uint32_t *x) {
+    if constexpr (N > 1) {
+        sort_falling<N / 2>(x);
+        sort_falling<N / 2>(x + N / 2);
+        // two falling halves: the larger of each mirrored pair first
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) order2(x[i], x[N - 1 - i]);
+        bitonic<N / 2>(x);
+        bitonic<N / 2>(x + N / 2);
+    }
+}
+// the KP largest of two falling lists
+template <int KP> __device__ __forceinline__ void merge_top(uint32_t *x, const uint32_t *y) {
+#pragma unroll
+    for (int i = 0; i < KP; i++) x[i] = x[i] > y[KP - 1 - i] ? x[i] : y[KP - 1 - i];
+    bitonic<KP>(x);
+}
+// the KP largest keys of a segment, falling, in every lane
+template <int L, int V, int KP> __device__ __forceinline__ void seg_top(const uint32_t *key, uint32_t *top) {
+    if constexpr (V <= KP) {
+#pragma unroll
+        for (int i = 0; i < KP; i++) top[i] = i < V ? key[i] : 0u;
+        sort_falling<V>(top);
+    } else {
+#pragma unroll
+        for (int i = 0; i < KP; i++) top[i] = key[i];
+        sort_falling<KP>(top);
+#pragma unroll
+        for (int b = KP; b < V; b += KP) {
+            uint32_t more[KP];
+#pragma unroll
+            for (int i = 0; i < KP; i++) more[i] = key[b + i];
+            sort_falling<KP>(more);
+            merge_top<KP>(top, more);
+        }
+    }
+    auto step = [&](auto I) {
+        uint32_t other[KP];
+#pragma unroll
+        for (int i = 0; i < KP; i++) other[i] = partner32<decltype(I)::value>(top[i]);
+        merge_top<KP>(top, other);
+    };
+    step(std::integral_constant<int, 0>());
+    step(std::integral_constant<int, 1>());
+    step(std::integral_constant<int, 2>());
+    step(std::integral_constant<int, 3>());
+    if constexpr (L == 64) {
+        step(std::integral_constant<int, 4>());
+        step(std::integral_constant<int, 5>());
+    }
+}
+
 constexpr double kDead = -INFINITY;   // an expert that cannot be chosen
 constexpr double kLast = -1e300;      // a live one whose choice value is no number: after all others
 
-// Places of a chunk's slots: rows of an expert in the order of the rows (bits of `mask`, one per
-// row of the chunk), slots without an expert after all experts' rows.
-__device__ __forceinline__ int32_t rank_in_chunk(const uint64_t *mask, int E, int e, int t) {
-    const int w = t >> 6;
-    int n = 0;
-    for (int i = 0; i < w; i++) n += __popcll(mask[i * E + e]);
-    return n + __popcll(mask[w * E + e] & ((1ull << (t & 63)) - 1));
+// Choice value of a live logit in 64 bits (m, sum: the row's softmax statistics).
+__device__ __forceinline__ double choice64(const RouteArgs &a, bool by_logit, float l, int e, float m, double sum) {
+    double x = (double)l;
+    if (!by_logit) {
+        x = a.score == 0 ? exp(x - (double)m) / sum : 1.0 / (1.0 + exp(-x));
+        if (a.bias) x += (double)a.bias[e];
+    }
+    return x >= kLast ? x : kLast;
+}
+
+// The choice of a row's experts from values in 64 bits, one at a time, by a whole wave: lane j's expert.
+// It is the definition of the choice, and what the 32-bit choice leaves to it where its values are too
+// close to tell the order, too far from the best, or no numbers.  value: E + G doubles of LDS (groups).
+template <int V>
+__device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, int lane, const float (&l)[V], float m,
+                                        double sum, double *value) {
+    const int E = a.E, G = a.groups, S = E / G;
+    double c[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int e = lane * V + v;
+        c[v] = e < E && l[v] != -INFINITY ? choice64(a, by_logit, l[v], e, m, sum) : kDead;
+    }
+    if (G > 1) {
+        double *score = value + E;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (lane * V + v < E) value[lane * V + v] = c[v];
+        wave_lds_sync();
+        double mine = kDead;
+        if (lane < G) {
+            double b2 = kDead;
+            for (int s = 0; s < S; s++) {
+                const double x = value[lane * S + s];
+                if (x > mine) { b2 = mine; mine = x; }
+                else if (x > b2) b2 = x;
+            }
+            if (a.group_sum == 2 && b2 > kDead) mine += b2;
+            score[lane] = mine;
+        }
+        wave_lds_sync();
+        int before = 0;         // a group is kept if fewer than top_groups come before it
+        for (int o = 0; o < G; o++) before += score[o] > mine || (score[o] == mine && o < lane);
+        const uint64_t kept = __ballot(lane < G && before < a.top_groups);
+        wave_lds_sync();
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int e = lane * V + v;
+            if (e < E && !((kept >> (e / S)) & 1)) c[v] = kDead;
+        }
+    }
+    int my_e = -1;
+    for (int j = 0; j < a.k; j++) {
+        double best = kDead;
+        int be = 1 << 20;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (c[v] > best) { best = c[v]; be = lane * V + v; }
+        auto join = [&](auto I) {
+            const double ob = partner<decltype(I)::value>(best);
+            const int oe = partner<decltype(I)::value>(be);
+            if (ob > best || (ob == best && oe < be)) { best = ob; be = oe; }
+        };
+        join(std::integral_constant<int, 0>());
+        join(std::integral_constant<int, 1>());
+        join(std::integral_constant<int, 2>());
+        join(std::integral_constant<int, 3>());
+        join(std::integral_constant<int, 4>());
+        join(std::integral_constant<int, 5>());
+        if (lane == j) my_e = best > kDead ? be : -1;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (lane * V + v == be) c[v] = kDead;
+    }
+    return my_e;
 }
 
 constexpr int kRouteThreads = 512;
-constexpr int kWords = kRouteChunk / 64;
-
-// Places of one chunk from its masks, the expert bases and the rows' slot counts; all threads.
-__device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int nt, const uint64_t *mask,
-                                            const int32_t *base, int32_t unused0, uint32_t *scan_tmp) {
-    // the chunk's slots without an expert, in order
-    const int t = threadIdx.x;
-    uint32_t un = 0;
-    if (t < nt)
-        for (int j = 0; j < a.k; j++) un += a.experts[(t0 + t) * a.k + j] < 0;
-    uint32_t total;
-    uint32_t at = block_excl_scan<kRouteThreads>(un, scan_tmp, total);
-    if (t < nt) {
-        for (int j = 0; j < a.k; j++) {
-            const int64_t slot = (t0 + t) * a.k + j;
-            const int e = a.experts[slot];
-            const int32_t p = e < 0 ? unused0 + (int32_t)at++ : base[e] + rank_in_chunk(mask, a.E, e, t);
-            a.pos[slot] = p;
-            a.src[p] = (int32_t)slot;
-        }
-    }
-}
 
 // Exclusive scan of v[0, E) in LDS by all threads; returns the total.
 __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tmp) {
@@ -189,204 +365,395 @@ __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tm
     return (int32_t)run;
 }
 
-template <typename T, int L, int V>
-__global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
+// Places of the slots of one chunk of 64 rows: rows of an expert in the order of the rows (mask[e]: the
+// chunk's rows that have it, base[e]: where its rows of this chunk begin), slots without an expert from
+// unused0 on.  All threads; `first` holds 64 words.
+__device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int nt, const uint64_t *mask,
+                                            const int32_t *base, int32_t unused0, uint32_t *first) {
+    const int k = a.k;
+    if (threadIdx.x < 64) {     // slots without an expert in the rows before
+        const int t = threadIdx.x;
+        uint32_t un = 0;
+        if (t < nt)
+            for (int j = 0; j < k; j++) un += a.experts[(t0 + t) * k + j] < 0;
+        const uint32_t incl = wave_incl_scan(un);
+        first[t] = incl - un - (k - un);        // + j = the slot's rank: they are a row's last slots
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nt * k; i += blockDim.x) {
+        const int t = i / k, j = i - t * k;
+        const int64_t slot = t0 * k + i;
+        const int e = a.experts[slot];
+        const int32_t p = e < 0 ? unused0 + (int32_t)(first[t] + j)
+                                : base[e] + __popcll(mask[e] & ((1ull << t) - 1));
+        a.pos[slot] = p;
+        a.src[p] = (int32_t)slot;
+    }
+}
+
+// Weights and outputs of a row (bit i of its chunk) with lane j's expert my_e, of which lanes < k hold
+// one; m, sum: the softmax statistics (scores not renormalised).  Softmax is exp(l - max) / sum,
+// renormalised over the chosen alone; the ratio of the chosen sigmoids comes from their logarithms,
+// which neither under- nor overflow.
+template <int L>
+__device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i, bool write, int lane, int my_e, bool nan,
+                                           float m, float sum, uint64_t *mask) {
+    float w = 0.f;
+    const bool used = my_e >= 0 && lane < a.k;
+    const float lw = used ? one_logit(a, t, my_e) : -INFINITY;
+    if (a.renorm) {
+        // (the logarithm is off by 2^-24 absolutely: its argument is in [1, 2])
+        const float z = !used ? -INFINITY : a.score == 0 ? lw
+                        : fminf(lw, 0.f) - 0.69314718f * __builtin_amdgcn_logf(1.f + fast_exp(-fabsf(lw)));
+        const float zm = seg_max<L>(z);
+        w = used ? fast_exp(z - zm) : 0.f;
+        const float ws = seg_reduce<L>(w, Sum());
+        w = used ? w / ws * a.scale : 0.f;
+    } else if (used) {
+        w = a.scale * (a.score == 0 ? fast_exp(lw - m) / sum : 1.f / (1.f + fast_exp(-lw)));
+    }
+    if (used && nan) w = NAN;
+    if (write && lane < a.k) {
+        a.experts[t * a.k + lane] = my_e;
+        a.weights[t * a.k + lane] = w;
+        if (my_e >= 0) atomicOr((unsigned long long *)&mask[my_e], 1ull << i);
+    }
+}
+
+// One workgroup routes a chunk of 64 rows, L lanes a row and V experts a lane.  The choice runs on
+// 32-bit keys that hold value and expert (unique, so that maxima need no ties): of 16-bit logits the
+// order-preserving bits themselves, else the value's distance from a floor below the row's best, in 24
+// bits (22 beyond 256 experts).  Sorting networks of the KP >= k largest keys run in registers and
+// across lanes.  A row where two neighbours of the result, or the last chosen and the first not, are
+// nearer than the keys' and the scores' error is left to choose64 after the others.
+template <int L, int V, int KP>
+__global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     extern __shared__ uint64_t lds[];
-    __shared__ uint32_t scan_tmp[kRouteThreads / 64];
-    const int E = a.E, k = a.k, G = a.groups;
-    uint64_t *mask = lds;                                             // [kWords][E]
-    double *choice = (double *)(mask + (size_t)kWords * E);           // [segments][E] (groups)
+    __shared__ uint32_t scan_tmp[kRouteThreads / 64], first[64];
+    __shared__ unsigned long long odd_rows;
+    constexpr int kIndex = L * V <= 256 ? 8 : 10;
+    constexpr uint32_t kIndexMask = (1u << kIndex) - 1, kExactMask = 0x1FFFu;
+    const int E = a.E, k = a.k, G = a.groups, S = E / G;
     const int lane = threadIdx.x & (L - 1), seg = threadIdx.x / L;
+    uint64_t *mask = lds;                                                  // [E]
+    double *room = (double *)(mask + E);                                   // groups alone:
+    float *score = (float *)room + (size_t)seg * G;                        // [segments][G]
+    float *value = (float *)room + (size_t)(kRouteThreads / L) * G + (size_t)seg * (L * V);  // [segments][L * V]
     const int64_t t0 = (int64_t)blockIdx.x * kRouteChunk;
     const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
-    for (int i = threadIdx.x; i < kWords * E; i += kRouteThreads) mask[i] = 0;
+    const bool by_logit = !a.bias && (G == 1 || a.group_sum == 1);
+    const bool exact = by_logit && a.dtype != 0;                           // keys that lose nothing
+    const bool exps = a.score == 0 && !(by_logit && a.renorm);             // softmax statistics wanted
+    const uint32_t inv = ((1u << 20) + S - 1) / S;                         // e / S = e * inv >> 20, e < 1024
+    for (int i = threadIdx.x; i < E; i += kRouteThreads) mask[i] = 0;
+    if (threadIdx.x == 0) odd_rows = 0;
+    float bias[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) bias[v] = 0.f;
+    if (a.bias) load(a.bias + lane * V, E - lane * V, bias);
     __syncthreads();
-    for (int i0 = 0; i0 < kRouteChunk; i0 += kRouteThreads / L) {
-        if (i0 >= nt) break;
+    for (int i0 = 0; i0 < nt; i0 += kRouteThreads / L) {
         const int i = i0 + seg;
         const bool row = i < nt;
         const int64_t t = t0 + (row ? i : 0);
-        const T *lp = (const T *)a.logits + t * a.ld;
         const bool on = row && (!a.valid || a.valid[t]);
-        float l[V];
-        load(lp + lane * V, E - lane * V, l);
-        // row statistics of the softmax
+        // c: -inf where the expert is masked
+        float c[V];
+        load_logits(a, t, lane * V, c);
         bool nan = false;
-        float m = -INFINITY;
+        float m = -INFINITY, sum = 1.f, eps = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; v++)
-            if (lane * V + v < E) { nan |= l[v] != l[v]; m = fmaxf(m, l[v]); }
-        nan = seg_reduce<L>((int)nan, [](int x, int y) { return x | y; });
-        m = seg_reduce<L>(m, [](float x, float y) { return fmaxf(x, y); });
-        double sum = 1.0;
-        if (a.score == 0) {
-            sum = 0.0;
+        for (int v = 0; v < V; v++) nan |= c[v] != c[v];
+        nan = seg_reduce<L>((int)nan, Or()) != 0;
+        if (a.score == 0 && (exps || !by_logit)) {
+#pragma unroll
+            for (int v = 0; v < V; v++) m = fmaxf(m, c[v]);
+            m = seg_max<L>(m);
+            const float mm = m == -INFINITY ? 0.f : m;
+            float s[V];
+            sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                s[v] = fast_exp(c[v] - mm);
+                sum += s[v];
+            }
+            sum = seg_reduce<L>(sum, Sum());
+            if (!by_logit) {
+                // off by 2e-6 at most: the exponent's rounding, and the sum over the row
+                eps = 2e-6f;
+                const float r = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+                for (int v = 0; v < V; v++) c[v] = c[v] == -INFINITY ? c[v] : fmaf(s[v], r, bias[v]);
+            }
+        } else if (!by_logit) {
+            // off by 5e-7: the exponent's rounding times s (1 - s), and a unit each of exp, sum, reciprocal
+            eps = 5e-7f;
 #pragma unroll
             for (int v = 0; v < V; v++)
-                if (lane * V + v < E && l[v] != -INFINITY) sum += exp((double)l[v] - (double)m);
-            sum = seg_reduce<L>(sum, [](double x, double y) { return x + y; });
+                c[v] = c[v] == -INFINITY ? c[v] : __builtin_amdgcn_rcpf(1.f + fast_exp(-c[v])) + bias[v];
         }
-        // choice values
-        const bool by_logit = !a.bias && (G == 1 || a.group_sum == 1);
-        double c[V];
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int e = lane * V + v;
-            c[v] = kDead;
-            if (e < E && on && l[v] != -INFINITY) {
-                double x = (double)l[v];
-                if (!by_logit) {
-                    x = a.score == 0 ? exp(x - (double)m) / sum : 1.0 / (1.0 + exp(-x));
-                    if (a.bias) x += (double)a.bias[e];
-                }
-                c[v] = x >= kLast ? x : kLast;
-            }
-        }
+        bool odd = false;
         if (G > 1) {
-            const int S = E / G;
-            double *mine = choice + (size_t)seg * E;
+            // the two best of every group: pairs in registers, then across lanes, or through LDS
+            if ((S & (S - 1)) == 0) {
+                float b1[V], b2[V];
 #pragma unroll
-            for (int v = 0; v < V; v++)
-                if (lane * V + v < E) mine[lane * V + v] = c[v];
-            wave_lds_sync();
-            double gs[kRouteMaxGroups / 16];
-            for (int n = 0, g = lane; g < G; n++, g += L) {
-                double b1 = kDead, b2 = kDead;
-                for (int s = 0; s < S; s++) {
-                    const double x = mine[g * S + s];
-                    if (x > b1) { b2 = b1; b1 = x; }
-                    else if (x > b2) b2 = x;
+                for (int v = 0; v < V; v++) { b1[v] = c[v]; b2[v] = -INFINITY; }
+#pragma unroll
+                for (int h = 1; h < V; h *= 2)
+                    if (h < S)
+#pragma unroll
+                        for (int v = 0; v < V; v += 2 * h) {
+                            const float lo = fminf(b1[v], b1[v + h]);
+                            b2[v] = fmaxf(lo, fmaxf(b2[v], b2[v + h]));
+                            b1[v] = fmaxf(b1[v], b1[v + h]);
+                        }
+                auto join = [&](auto I) {
+                    if ((V << decltype(I)::value) < S) {
+                        const float o1 = partner<decltype(I)::value>(b1[0]), o2 = partner<decltype(I)::value>(b2[0]);
+                        b2[0] = fmaxf(fminf(b1[0], o1), fmaxf(b2[0], o2));
+                        b1[0] = fmaxf(b1[0], o1);
+                    }
+                };
+                join(std::integral_constant<int, 0>());
+                join(std::integral_constant<int, 1>());
+                join(std::integral_constant<int, 2>());
+                join(std::integral_constant<int, 3>());
+                if constexpr (L == 64) {
+                    join(std::integral_constant<int, 4>());
+                    join(std::integral_constant<int, 5>());
                 }
-                if (a.group_sum == 2 && b2 > kDead) b1 += b2;
-                gs[n] = b1;
+#pragma unroll
+                for (int v = 0; v < V; v++)
+                    if ((v & (S - 1)) == 0 && ((lane * V) & (S - 1)) == 0 && lane * V + v < E)
+                        score[((uint32_t)(lane * V + v) * inv) >> 20] =
+                            a.group_sum == 2 && b2[v] > -INFINITY ? b1[v] + b2[v] : b1[v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; v++) value[lane * V + v] = c[v];
+                wave_lds_sync();
+                for (int g = lane; g < G; g += L) {
+                    float b1 = -INFINITY, b2 = -INFINITY;
+                    for (int s = 0; s < S; s++) {
+                        const float x = value[g * S + s];
+                        b2 = fmaxf(b2, fminf(b1, x));
+                        b1 = fmaxf(b1, x);
+                    }
+                    score[g] = a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+                }
             }
             wave_lds_sync();
-            for (int n = 0, g = lane; g < G; n++, g += L) mine[g] = gs[n];
-            wave_lds_sync();
-            uint64_t kept = 0;      // groups kept: fewer than top_groups come before them
+            uint64_t kept = 0;
+            float least = INFINITY, most = -INFINITY;     // of the groups kept, and of the others
             for (int g = lane; g < G; g += L) {
-                const double x = mine[g];
+                const float x = score[g];
                 int before = 0;
-                for (int o = 0; o < G; o++) before += mine[o] > x || (mine[o] == x && o < g);
-                if (before < a.top_groups) kept |= 1ull << g;
+#pragma unroll 4
+                for (int o = 0; o < G; o++) {
+                    const float y = score[o];
+                    before += y > x || (y == x && o < g);
+                }
+                if (before < a.top_groups) {
+                    kept |= 1ull << g;
+                    least = fminf(least, x);
+                } else {
+                    most = fmaxf(most, x);
+                }
             }
-            kept = seg_reduce<L>(kept, [](uint64_t x, uint64_t y) { return x | y; });
+            kept = seg_reduce<L>(kept, Or());
+            if (!by_logit) {
+                least = seg_min<L>(least);
+                most = seg_max<L>(most);
+                // two scores' errors on either side, and the roundings of their sums
+                odd = most > -INFINITY &&
+                      !(least - most > 4.f * eps + 8.f * 0x1p-24f * fmaxf(fabsf(least), fabsf(most)));
+            }
             wave_lds_sync();
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const int e = lane * V + v;
-                if (e < E && !((kept >> (e / S)) & 1)) c[v] = kDead;
+                const uint32_t g = ((uint32_t)(lane * V + v) * inv) >> 20;
+                c[v] = kept >> (g & 63) & 1 ? c[v] : -INFINITY;
             }
         }
-        // the k best, ties to the lowest index; lane j keeps the j-th
-        int my_e = -1;
-        for (int j = 0; j < k; j++) {
-            double best = kDead;
-            int be = 1 << 20;
+        uint32_t key[V];
+        if (exact) {
 #pragma unroll
-            for (int v = 0; v < V; v++)
-                if (c[v] > best) { best = c[v]; be = lane * V + v; }
-#pragma unroll
-            for (int s = L / 2; s; s >>= 1) {
-                const double ob = __shfl_xor(best, s, 64);
-                const int oe = __shfl_xor(be, s, 64);
-                if (ob > best || (ob == best && oe < be)) { best = ob; be = oe; }
+            for (int v = 0; v < V; v++) {
+                uint32_t u = __float_as_uint(c[v] + 0.f);       // -0 is 0
+                u ^= (uint32_t)((int32_t)u >> 31) | 0x80000000u;
+                u = (u & ~kExactMask) | (kExactMask - (lane * V + v));
+                key[v] = c[v] == -INFINITY ? 0u : u;
             }
-            if (lane == j) my_e = best > kDead ? be : -1;
+        } else {
+            float top = -INFINITY;
 #pragma unroll
-            for (int v = 0; v < V; v++)
-                if (lane * V + v == be) c[v] = kDead;
+            for (int v = 0; v < V; v++) top = fmaxf(top, c[v]);
+            top = seg_max<L>(top);
+            // scores span less than 2 unless a bias does more; values at or below the floor have key 0
+            // and, where one of them is chosen, choose64 tells them apart and from masked ones
+            constexpr float kSteps = (float)((1 << (32 - kIndex)) - 8);
+            const float scale = by_logit ? kSteps / 16.f : kSteps / 2.f;
+            odd |= !(fabsf(top) < 1e6f) && top > -INFINITY;
+            eps = 2.f * scale * (eps > 0.f ? eps + 0x1p-23f * fmaxf(fabsf(top), 1.f) : 0.f) + 4.f;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const uint32_t q = (uint32_t)fmaxf(fmaf(c[v] - top, scale, kSteps), 0.f);
+                key[v] = q << kIndex | (kIndexMask - (uint32_t)(lane * V + v));
+            }
         }
-        // weights: softmax as exp(l - max) / sum, renormalised over the chosen alone; the chosen
-        // sigmoids' ratio from their logarithms, which neither under- nor overflow
-        float w = 0.f;
-        const bool used = my_e >= 0 && lane < k;
-        const float lw = used ? Value<T>::up(lp[my_e]) : -INFINITY;
-        if (a.renorm) {
-            const float z = !used ? -INFINITY : a.score == 0 ? lw : fminf(lw, 0.f) - log1pf(expf(-fabsf(lw)));
-            const float zm = seg_reduce<L>(z, [](float x, float y) { return fmaxf(x, y); });
-            w = used ? expf(z - zm) : 0.f;
-            const float ws = seg_reduce<L>(w, [](float x, float y) { return x + y; });
-            w = used ? w / ws * a.scale : 0.f;
-        } else if (used) {
-            w = a.scale * (a.score == 0 ? expf(lw - m) / (float)sum : 1.f / (1.f + expf(-lw)));
+        uint32_t top[KP];
+        seg_top<L, V, KP>(key, top);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < KP; j++) mine = lane == j ? top[j] : mine;
+        int my_e;
+        if (exact) {
+            my_e = mine ? (int)(kExactMask - (mine & kExactMask)) : -1;
+            odd = nan;
+        } else {
+            my_e = (int)(kIndexMask - (mine & kIndexMask));
+            // neighbours nearer than eps, or one at the floor; then the best key that was not chosen
+            uint32_t last = 0;
+#pragma unroll
+            for (int j = 0; j < KP; j++) {
+                const uint32_t q = top[j] >> kIndex;
+                if (j < k) {
+                    if (j) odd |= (float)((last >> kIndex) - q) < eps;
+                    odd |= q == 0;
+                    last = top[j];
+                }
+            }
+            uint32_t rest = 0;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const uint32_t x = key[v] < last ? key[v] : 0u;
+                rest = x > rest ? x : rest;
+            }
+            rest = seg_reduce<L>(rest, Max());
+            odd |= (float)((last >> kIndex) - (rest >> kIndex)) < eps;
+            odd |= nan;
         }
-        if (used && nan) w = NAN;
-        if (row && lane < k) {
-            a.experts[t * k + lane] = my_e;
-            a.weights[t * k + lane] = w;
-            if (my_e >= 0) atomicOr((unsigned long long *)&mask[(i >> 6) * E + my_e], 1ull << (i & 63));
-        }
+        odd = odd && on;
+        if (!on || lane >= k) my_e = -1;
+        if (odd && lane == 0) atomicOr(&odd_rows, 1ull << i);
+        finish_row<L>(a, t, i, row && !odd, lane, my_e, nan, m, sum, mask);
     }
     __syncthreads();
-    if (a.hist) {
-        for (int e = threadIdx.x; e < E; e += kRouteThreads) {
-            int n = 0;
-            for (int w = 0; w < kWords; w++) n += __popcll(mask[w * E + e]);
-            a.hist[(int64_t)blockIdx.x * E + e] = (uint16_t)n;
+    // the rows left, a wave each
+    constexpr int VX = L == 64 ? V : (V + 3) / 4;
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
+    const int odds = __popcll(odd_rows);
+    for (int n0 = wave; n0 < odds; n0 += kRouteThreads / 64) {
+        unsigned long long left = odd_rows;
+        for (int n = 0; n < n0; n++) left &= left - 1;
+        const int i = __ffsll(left) - 1;
+        const int64_t t = t0 + i;
+        float l[VX];
+        load_logits(a, t, wl * VX, l);
+        bool nan = false;
+        float m = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < VX; v++) {
+            nan |= l[v] != l[v];
+            m = fmaxf(m, l[v]);
         }
+        nan = seg_reduce<64>((int)nan, Or()) != 0;
+        m = seg_max<64>(m);
+        double sum = 1.0;
+        if (exps) {
+            sum = 0.0;
+#pragma unroll
+            for (int v = 0; v < VX; v++)
+                if (l[v] != -INFINITY) sum += exp((double)l[v] - (double)m);
+            sum = seg_reduce<64>(sum, Sum());
+        }
+        const int my_e = choose64<VX>(a, by_logit, wl, l, m, sum, room + (size_t)wave * (E + G));
+        finish_row<64>(a, t, i, true, wl, my_e, nan, m, (float)sum, mask);
+    }
+    __syncthreads();
+    if (a.mask) {
+        for (int e = threadIdx.x; e < E; e += kRouteThreads) a.mask[(int64_t)blockIdx.x * E + e] = mask[e];
         return;
     }
     // the only chunk: places at once
-    int32_t *base = (int32_t *)(mask + (size_t)kWords * E);
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
-        int n = 0;
-        for (int w = 0; w < kWords; w++) n += __popcll(mask[w * E + e]);
-        base[e] = n;
-    }
+    int32_t *base = (int32_t *)(mask + E);
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) base[e] = __popcll(mask[e]);
     __syncthreads();
     const int32_t total = scan_lds(base, E, scan_tmp);
     for (int e = threadIdx.x; e < E; e += kRouteThreads) a.offsets[e] = base[e];
     if (threadIdx.x == 0) a.offsets[E] = total;
-    place_chunk(a, t0, nt, mask, base, total, scan_tmp);
+    place_chunk(a, t0, nt, mask, base, total, first);
 }
 
-// Places of every chunk: each workgroup sums the chunks' counts before its own and in all.
-__global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, int64_t chunks) {
-    extern __shared__ uint64_t lds[];
-    __shared__ uint32_t scan_tmp[kRouteThreads / 64];
-    const int E = a.E, k = a.k;
-    uint64_t *mask = lds;                                    // [kWords][E]
-    int32_t *base = (int32_t *)(mask + (size_t)kWords * E);  // [E] all counts, then the bases
-    int32_t *prev = base + E;                                // [E] counts of the chunks before
-    const int64_t c = blockIdx.x, t0 = c * kRouteChunk;
-    const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
-    for (int i = threadIdx.x; i < kWords * E; i += kRouteThreads) mask[i] = 0;
-    for (int e = threadIdx.x; e < 2 * E; e += kRouteThreads) base[e] = 0;
+// Rows of every expert in the chunks before each chunk, and in all chunks: a workgroup takes 8 experts,
+// 128 threads of each over the chunks (two passes; the masks of the second come from L2).
+__global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict__ mask, int32_t *__restrict__ before,
+                                                     int32_t *__restrict__ total, int64_t chunks, int E) {
+    __shared__ int32_t part[8][129];
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3, e = blockIdx.x * 8 + x;
+    const int64_t per = (chunks + 127) / 128, lo = y * per, hi = lo + per < chunks ? lo + per : chunks;
+    int32_t n = 0;
+    if (e < E) {
+#pragma unroll 8
+        for (int64_t c = lo; c < hi; c++) n += __popcll(mask[c * E + e]);
+    }
+    part[x][y] = n;
     __syncthreads();
-    // threads share the experts; with few experts several threads share one, over the chunks
-    const int per = E >= kRouteThreads ? 1 : kRouteThreads / E;
-    const int part = E >= kRouteThreads ? 0 : threadIdx.x / E;
-    if (part < per) {
-        for (int e = E >= kRouteThreads ? threadIdx.x : threadIdx.x % E; e < E; e += kRouteThreads) {
-            int32_t before = 0, all = 0;
-            for (int64_t b = part; b < chunks; b += per) {
-                const int32_t n = a.hist[b * E + e];
-                all += n;
-                before += b < c ? n : 0;
-            }
-            atomicAdd(&base[e], all);
-            atomicAdd(&prev[e], before);
+    // a wave per expert scans its 128 parts
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (w < 8) {
+        const int32_t p = part[w][2 * lane], q = part[w][2 * lane + 1];
+        const int32_t incl = (int32_t)wave_incl_scan((uint32_t)(p + q));
+        part[w][2 * lane] = incl - p - q;
+        part[w][2 * lane + 1] = incl - q;
+        if (lane == 63 && blockIdx.x * 8 + w < E) total[blockIdx.x * 8 + w] = incl;
+    }
+    __syncthreads();
+    if (e < E) {
+        n = part[x][y];
+#pragma unroll 8
+        for (int64_t c = lo; c < hi; c++) {
+            const int32_t rows = __popcll(mask[c * E + e]);
+            before[c * E + e] = n;
+            n += rows;
         }
     }
-    for (int i = threadIdx.x; i < nt * k; i += kRouteThreads) {
-        const int e = a.experts[t0 * k + i], t = i / k;
-        if (e >= 0) atomicOr((unsigned long long *)&mask[(t >> 6) * E + e], 1ull << (t & 63));
+}
+
+// Places of one chunk's slots.
+__global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
+                                                               const int32_t *__restrict__ totals) {
+    extern __shared__ uint64_t lds[];
+    __shared__ uint64_t scan_tmp[kRouteThreads / 64];
+    __shared__ uint32_t first[64];
+    const int E = a.E;
+    uint64_t *mask = lds;                       // [E]
+    int32_t *base = (int32_t *)(mask + E);      // [E]
+    const int64_t c = blockIdx.x, t0 = c * kRouteChunk;
+    const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
+    // exclusive sums over the experts: all their rows, and (high half) this chunk's predecessors' rows
+    uint64_t run = 0;
+    for (int e0 = 0; e0 < E; e0 += kRouteThreads) {
+        const int e = e0 + threadIdx.x;
+        uint32_t all = 0, prev = 0;
+        if (e < E) {
+            mask[e] = a.mask[c * E + e];
+            all = (uint32_t)totals[e];
+            prev = (uint32_t)before[c * E + e];
+        }
+        uint64_t sum;
+        const uint64_t pre = run + block_excl_scan<kRouteThreads>((uint64_t)prev << 32 | all, scan_tmp, sum);
+        run += sum;
+        if (e < E) {
+            base[e] = (int32_t)((uint32_t)pre + prev);
+            if (c == 0) a.offsets[e] = (int32_t)(uint32_t)pre;
+        }
     }
+    const int32_t total = (int32_t)(uint32_t)run, used_all = (int32_t)(run >> 32);
+    if (c == 0 && threadIdx.x == 0) a.offsets[E] = total;
     __syncthreads();
-    const int32_t total = scan_lds(base, E, scan_tmp);
-    if (c == 0) {
-        for (int e = threadIdx.x; e < E; e += kRouteThreads) a.offsets[e] = base[e];
-        if (threadIdx.x == 0) a.offsets[E] = total;
-    }
-    // slots without an expert in the chunks before
-    uint32_t used = 0, used_all;
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) used += prev[e];
-    block_excl_scan<kRouteThreads>(used, scan_tmp, used_all);
-    __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) base[e] += prev[e];
-    __syncthreads();
-    place_chunk(a, t0, nt, mask, base, (int32_t)(total + t0 * k - used_all), scan_tmp);
+    // slots without an expert in the chunks before: all of theirs less the used ones
+    place_chunk(a, t0, nt, mask, base, (int32_t)(total + t0 * a.k - used_all), first);
 }
 
 // dlogits of one row from the chosen slots' gradients: with a = w / scale,
@@ -413,7 +780,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const
             e = a.experts[tt * k + lane];
             if (e >= 0) { w = a.weights[tt * k + lane]; g = dweights[tt * k + lane]; }
         }
-        const float dot = seg_reduce<L>(g * w, [](float x, float y) { return x + y; });
+        const float dot = seg_reduce<L>(g * w, Sum());
         float x = w * (a.renorm ? g - dot / a.scale : g);
         if (a.score == 1 && e >= 0) x /= 1.f + expf(Value<T>::up(lp[e]));
 #pragma unroll
@@ -431,14 +798,14 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const
 #pragma unroll
             for (int v = 0; v < V; v++)
                 if (lane * V + v < E) m = fmaxf(m, l[v]);
-            m = seg_reduce<L>(m, [](float p, float q) { return fmaxf(p, q); });
+            m = seg_max<L>(m);
             float s[V];
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 s[v] = lane * V + v < E && l[v] != -INFINITY ? expf(l[v] - m) : 0.f;
                 sum += s[v];
             }
-            sum = seg_reduce<L>(sum, [](float p, float q) { return p + q; });
+            sum = seg_reduce<L>(sum, Sum());
             const float f = sum != 0.f ? dot / sum : 0.f;
 #pragma unroll
             for (int v = 0; v < V; v++)
@@ -586,7 +953,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
         }
         if (!dw) continue;
 #pragma unroll
-        for (int j = 0; j < KM; j++) dot[j] = seg_reduce<(L < 64 ? L : 64)>(dot[j], [](float a, float b) { return a + b; });
+        for (int j = 0; j < KM; j++) dot[j] = seg_reduce<(L < 64 ? L : 64)>(dot[j], Sum());
         if (L > 64) {
             __syncthreads();
             if ((threadIdx.x & 63) == 0)
@@ -699,22 +1066,31 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
 
 hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
     const int64_t chunks = route_chunks(a.T);
-    hipError_t err = hipSuccess;
-    const hipError_t e = by_type(a.dtype, [&](auto *p) {
-        using T = std::remove_pointer_t<decltype(p)>;
-        by_width(a.E, [&](auto L, auto V) {
-            size_t lds = 8 * (size_t)kWords * a.E + 4 * (size_t)a.E;
-            if (a.groups > 1) lds = 8 * (size_t)kWords * a.E + 8 * (size_t)(kRouteThreads / L) * a.E;
-            auto kern = k_route<T, decltype(L)::value, decltype(V)::value>;
-            if (lds > 64 * 1024)
-                err = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (err == hipSuccess) hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kRouteThreads), lds, s, a);
-        });
+    const int S = a.E / a.groups;
+    by_width(a.E, [&](auto L, auto V) {
+        // masks; the bases (one chunk); with groups their scores and, for groups of no power of two, the
+        // values of every row at once, or the values and scores in 64 bits of a row for every wave
+        const size_t rows = kRouteThreads / decltype(L)::value, E = a.E, G = a.groups;
+        size_t room = 4 * E;
+        if (G > 1) {
+            room = std::max(room, rows * 4 * (G + (S & (S - 1) ? (size_t)(L * V) : 0)));
+            room = std::max(room, kRouteThreads / 64 * 8 * (E + G));
+        }
+        const size_t lds = 8 * E + room;
+        auto go = [&](auto KP) {
+            hipLaunchKernelGGL((k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value>),
+                               dim3((unsigned)chunks), dim3(kRouteThreads), lds, s, a);
+        };
+        if (a.k <= 4) go(std::integral_constant<int, 4>());
+        else if (a.k <= 8) go(std::integral_constant<int, 8>());
+        else go(std::integral_constant<int, 16>());
     });
-    if (err != hipSuccess) return err;
-    if (e != hipSuccess || chunks == 1) return e;
-    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads),
-                       8 * (size_t)kWords * a.E + 8 * (size_t)a.E, s, a, chunks);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.mask) return e;
+    hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 7) / 8)), dim3(1024), 0, s, a.mask, a.before, a.totals,
+                       chunks, a.E);
+    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads), 12 * (size_t)a.E, s, a, a.before,
+                       a.totals);
     return hipGetLastError();
 }
 

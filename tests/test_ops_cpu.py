@@ -237,7 +237,7 @@ def test_other_entries_refuse_on_the_host():
     assert lib.pss_route_grad(None, 8, 4, 8, 2, 0, 0, 1, 1.0, None, None, None, None, None) == 1
     # handles: no sampler, no epoch
     assert lib.pss_gather_dropout(None, None, 0, 8, None, None, None, 0, 0.5, 0, 0, None, 0, None, None) == 1
-    assert lib.pss_route_workspace(256, 64) == 0 and lib.pss_route_workspace(257, 64) > 0
+    assert lib.pss_route_workspace(64, 64) == 0 and lib.pss_route_workspace(65, 64) > 0
     assert lib.pss_route_workspace(-1, 64) == 0
     v = ctypes.c_uint64()
     assert lib.pss_dropout_key(1, 2, 3, 4, ctypes.byref(v)) == 0 and v.value == ops.dropout_key(1, 2, 3, 4)
