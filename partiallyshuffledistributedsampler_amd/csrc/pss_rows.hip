@@ -233,8 +233,9 @@ template <int KP> __device__ __forceinline__ void merge_top(uint32_t *x, const u
     for (int i = 0; i < KP; i++) x[i] = x[i] > y[KP - 1 - i] ? x[i] : y[KP - 1 - i];
     bitonic<KP>(x);
 }
-// the KP largest keys of a segment, falling, in every lane
-template <int L, int V, int KP> __device__ __forceinline__ void seg_top(const uint32_t *key, uint32_t *top) {
+// the KP largest keys of a segment, falling, in every lane; each lane's less `first` (0 stays 0)
+template <int L, int V, int KP>
+__device__ __forceinline__ void seg_top(const uint32_t *key, uint32_t first, uint32_t *top) {
     if constexpr (V <= KP) {
 #pragma unroll
         for (int i = 0; i < KP; i++) top[i] = i < V ? key[i] : 0u;
@@ -252,6 +253,8 @@ template <int L, int V, int KP> __device__ __forceinline__ void seg_top(const ui
             merge_top<KP>(top, more);
         }
     }
+#pragma unroll
+    for (int i = 0; i < KP; i++) top[i] = top[i] ? top[i] - first : 0u;
     auto step = [&](auto I) {
         uint32_t other[KP];
 #pragma unroll
@@ -270,6 +273,14 @@ template <int L, int V, int KP> __device__ __forceinline__ void seg_top(const ui
 
 constexpr double kDead = -INFINITY;   // an expert that cannot be chosen
 constexpr double kLast = -1e300;      // a live one whose choice value is no number: after all others
+
+// the maximum of a wave: inside rows of 16 lanes, then of the four rows
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = seg_reduce<16>(v, Max());
+    const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+    const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+    return std::max(std::max(a, b), std::max(c, d));
+}
 
 // Choice value of a live logit in 64 bits (m, sum: the row's softmax statistics).
 __device__ __forceinline__ double choice64(const RouteArgs &a, bool by_logit, float l, int e, float m, double sum) {
@@ -303,17 +314,22 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, int l
         double mine = kDead;
         if (lane < G) {
             double b2 = kDead;
+#pragma unroll 4
             for (int s = 0; s < S; s++) {
                 const double x = value[lane * S + s];
-                if (x > mine) { b2 = mine; mine = x; }
-                else if (x > b2) b2 = x;
+                b2 = x > mine ? mine : x > b2 ? x : b2;
+                mine = x > mine ? x : mine;
             }
             if (a.group_sum == 2 && b2 > kDead) mine += b2;
             score[lane] = mine;
         }
         wave_lds_sync();
         int before = 0;         // a group is kept if fewer than top_groups come before it
-        for (int o = 0; o < G; o++) before += score[o] > mine || (score[o] == mine && o < lane);
+#pragma unroll 4
+        for (int o = 0; o < G; o++) {
+            const double x = score[o];
+            before += x > mine || (x == mine && o < lane);
+        }
         const uint64_t kept = __ballot(lane < G && before < a.top_groups);
         wave_lds_sync();
 #pragma unroll
@@ -325,25 +341,26 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, int l
     int my_e = -1;
     for (int j = 0; j < a.k; j++) {
         double best = kDead;
-        int be = 1 << 20;
+        int be = -1;
 #pragma unroll
         for (int v = 0; v < V; v++)
             if (c[v] > best) { best = c[v]; be = lane * V + v; }
-        auto join = [&](auto I) {
-            const double ob = partner<decltype(I)::value>(best);
-            const int oe = partner<decltype(I)::value>(be);
-            if (ob > best || (ob == best && oe < be)) { best = ob; be = oe; }
-        };
-        join(std::integral_constant<int, 0>());
-        join(std::integral_constant<int, 1>());
-        join(std::integral_constant<int, 2>());
-        join(std::integral_constant<int, 3>());
-        join(std::integral_constant<int, 4>());
-        join(std::integral_constant<int, 5>());
-        if (lane == j) my_e = best > kDead ? be : -1;
+        // the wave's maximum as ordered bits, high word first; of equal values the lowest lane's
+        uint64_t u;
+        best += 0.0;            // -0 is 0
+        __builtin_memcpy(&u, &best, 8);
+        u ^= (uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull;
+        const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u, top = wave_max(hi);
+        uint64_t who = __ballot(hi == top);
+        if (who & (who - 1)) {
+            const uint32_t low = wave_max(hi == top ? lo : 0u);
+            who = __ballot(hi == top && lo == low);
+        }
+        const int won = __builtin_amdgcn_readlane(be, __builtin_ctzll(who));    // -1: none is left
+        if (lane == j) my_e = won;
 #pragma unroll
         for (int v = 0; v < V; v++)
-            if (lane * V + v == be) c[v] = kDead;
+            if (lane * V + v == won) c[v] = kDead;
     }
     return my_e;
 }
@@ -434,7 +451,8 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     constexpr int kIndex = L * V <= 256 ? 8 : 10;
     constexpr uint32_t kIndexMask = (1u << kIndex) - 1, kExactMask = 0x1FFFu;
     const int E = a.E, k = a.k, G = a.groups, S = E / G;
-    const int lane = threadIdx.x & (L - 1), seg = threadIdx.x / L;
+    int lane = threadIdx.x & (L - 1);
+    const int seg = threadIdx.x / L;
     uint64_t *mask = lds;                                                  // [E]
     double *room = (double *)(mask + E);                                   // groups alone:
     float *score = (float *)room + (size_t)seg * G;                        // [segments][G]
@@ -447,12 +465,21 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     const uint32_t inv = ((1u << 20) + S - 1) / S;                         // e / S = e * inv >> 20, e < 1024
     for (int i = threadIdx.x; i < E; i += kRouteThreads) mask[i] = 0;
     if (threadIdx.x == 0) odd_rows = 0;
-    float bias[V];
+    // (in LDS, value v of lane x at v / 4 * 4 * L + 4 * x + v % 4: registers are what limits the waves)
+    __shared__ float bias[L * V < 64 ? 64 : L * V];
+    constexpr int kVec = V < 4 ? V : 4;
+    if (a.bias)
+        for (int e = threadIdx.x; e < L * V; e += kRouteThreads) {
+            const int x = e / V, v = e % V;
+            bias[(v / kVec * L + x) * kVec + v % kVec] = e < E ? a.bias[e] : 0.f;
+        }
+    auto add_bias = [&](float (&c)[V]) {
 #pragma unroll
-    for (int v = 0; v < V; v++) bias[v] = 0.f;
-    if (a.bias) load(a.bias + lane * V, E - lane * V, bias);
+        for (int v = 0; v < V; v++) c[v] += bias[(v / kVec * L + lane) * kVec + v % kVec];
+    };
     __syncthreads();
     for (int i0 = 0; i0 < nt; i0 += kRouteThreads / L) {
+        asm volatile("" : "+v"(lane));      // what depends on the lane is made anew for every row, not kept
         const int i = i0 + seg;
         const bool row = i < nt;
         const int64_t t = t0 + (row ? i : 0);
@@ -483,36 +510,39 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                 eps = 2e-6f;
                 const float r = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
-                for (int v = 0; v < V; v++) c[v] = c[v] == -INFINITY ? c[v] : fmaf(s[v], r, bias[v]);
+                for (int v = 0; v < V; v++) c[v] = c[v] == -INFINITY ? c[v] : s[v] * r;
+                if (a.bias) add_bias(c);
             }
         } else if (!by_logit) {
             // off by 5e-7: the exponent's rounding times s (1 - s), and a unit each of exp, sum, reciprocal
             eps = 5e-7f;
 #pragma unroll
             for (int v = 0; v < V; v++)
-                c[v] = c[v] == -INFINITY ? c[v] : __builtin_amdgcn_rcpf(1.f + fast_exp(-c[v])) + bias[v];
+                c[v] = c[v] == -INFINITY ? c[v] : __builtin_amdgcn_rcpf(1.f + fast_exp(-c[v]));
+            if (a.bias) add_bias(c);
         }
         bool odd = false;
         if (G > 1) {
-            // the two best of every group: pairs in registers, then across lanes, or through LDS
+            // the two best of every group: a lane's values one by one, then across lanes, or through LDS
             if ((S & (S - 1)) == 0) {
-                float b1[V], b2[V];
+                float b1 = -INFINITY, b2 = -INFINITY;
+                auto flush = [&](int e) {       // of the group that ends with expert e
+                    score[((uint32_t)e * inv) >> 20] = a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+                };
 #pragma unroll
-                for (int v = 0; v < V; v++) { b1[v] = c[v]; b2[v] = -INFINITY; }
-#pragma unroll
-                for (int h = 1; h < V; h *= 2)
-                    if (h < S)
-#pragma unroll
-                        for (int v = 0; v < V; v += 2 * h) {
-                            const float lo = fminf(b1[v], b1[v + h]);
-                            b2[v] = fmaxf(lo, fmaxf(b2[v], b2[v + h]));
-                            b1[v] = fmaxf(b1[v], b1[v + h]);
-                        }
+                for (int v = 0; v < V; v++) {
+                    b2 = __builtin_amdgcn_fmed3f(b1, b2, c[v]);
+                    b1 = fmaxf(b1, c[v]);
+                    if (((v + 1) & (S - 1)) == 0) {
+                        if (lane * V + v < E) flush(lane * V + v);
+                        b1 = b2 = -INFINITY;
+                    }
+                }
                 auto join = [&](auto I) {
                     if ((V << decltype(I)::value) < S) {
-                        const float o1 = partner<decltype(I)::value>(b1[0]), o2 = partner<decltype(I)::value>(b2[0]);
-                        b2[0] = fmaxf(fminf(b1[0], o1), fmaxf(b2[0], o2));
-                        b1[0] = fmaxf(b1[0], o1);
+                        const float o1 = partner<decltype(I)::value>(b1), o2 = partner<decltype(I)::value>(b2);
+                        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+                        b1 = fmaxf(b1, o1);
                     }
                 };
                 join(std::integral_constant<int, 0>());
@@ -523,11 +553,7 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                     join(std::integral_constant<int, 4>());
                     join(std::integral_constant<int, 5>());
                 }
-#pragma unroll
-                for (int v = 0; v < V; v++)
-                    if ((v & (S - 1)) == 0 && ((lane * V) & (S - 1)) == 0 && lane * V + v < E)
-                        score[((uint32_t)(lane * V + v) * inv) >> 20] =
-                            a.group_sum == 2 && b2[v] > -INFINITY ? b1[v] + b2[v] : b1[v];
+                if (S > V && ((lane * V) & (S - 1)) == 0 && lane * V < E) flush(lane * V);
             } else {
 #pragma unroll
                 for (int v = 0; v < V; v++) value[lane * V + v] = c[v];
@@ -569,19 +595,25 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                       !(least - most > 4.f * eps + 8.f * 0x1p-24f * fmaxf(fabsf(least), fabsf(most)));
             }
             wave_lds_sync();
+            const uint32_t g0 = ((uint32_t)(lane * V) * inv) >> 20;
+            const uint32_t from = (uint32_t)(kept >> (g0 & 63));           // bit 0: the first value's group
+            if (S >= V && (S & (S - 1)) == 0) {
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                const uint32_t g = ((uint32_t)(lane * V + v) * inv) >> 20;
-                c[v] = kept >> (g & 63) & 1 ? c[v] : -INFINITY;
+                for (int v = 0; v < V; v++) c[v] = from & 1 ? c[v] : -INFINITY;
+            } else {
+                const uint32_t r0 = lane * V - g0 * S;
+#pragma unroll
+                for (int v = 0; v < V; v++) c[v] = from >> (((r0 + v) * inv) >> 20) & 1 ? c[v] : -INFINITY;
             }
         }
+        // (a key holds the place in the lane until the lane's own are sorted: fewer registers)
         uint32_t key[V];
         if (exact) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 uint32_t u = __float_as_uint(c[v] + 0.f);       // -0 is 0
                 u ^= (uint32_t)((int32_t)u >> 31) | 0x80000000u;
-                u = (u & ~kExactMask) | (kExactMask - (lane * V + v));
+                u = (u & ~kExactMask) | (kExactMask - v);
                 key[v] = c[v] == -INFINITY ? 0u : u;
             }
         } else {
@@ -598,11 +630,11 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 const uint32_t q = (uint32_t)fmaxf(fmaf(c[v] - top, scale, kSteps), 0.f);
-                key[v] = q << kIndex | (kIndexMask - (uint32_t)(lane * V + v));
+                key[v] = q << kIndex | (kIndexMask - v);
             }
         }
         uint32_t top[KP];
-        seg_top<L, V, KP>(key, top);
+        seg_top<L, V, KP>(key, lane * V, top);
         uint32_t mine = 0;
 #pragma unroll
         for (int j = 0; j < KP; j++) mine = lane == j ? top[j] : mine;
@@ -624,9 +656,10 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                 }
             }
             uint32_t rest = 0;
+            const uint32_t below = last + lane * V;
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const uint32_t x = key[v] < last ? key[v] : 0u;
+                const uint32_t x = key[v] < below ? key[v] : 0u;
                 rest = x > rest ? x : rest;
             }
             rest = seg_reduce<L>(rest, Max());

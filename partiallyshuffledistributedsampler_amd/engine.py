@@ -176,16 +176,23 @@ class IndexEngine:
         if out is None:
             out = torch.empty((n,) + tuple(data.shape[1:]), dtype=data.dtype, device=d)
         if p:
-            from .ops import DTYPES, _p, _row_ids
+            from .ops import DTYPES, _row_ids
             if data.dtype not in DTYPES:
                 raise TypeError("gather with dropout needs float32, bfloat16 or float16 data, got %s" % data.dtype)
             if not (out.is_contiguous() and out.dtype == data.dtype and out.device == d
                     and out.numel() >= n * (row_bytes // data.element_size())):
                 raise ValueError("gather: out must be contiguous, of the data's dtype, on the engine's device")
-            row0, ids = _row_ids(rows, n, d)
+            if not 0.0 <= p <= 1.0:
+                raise ValueError("p must be in [0, 1], got %r" % p)
+            row0, ids = _row_ids(rows)
+            if ids is not None:
+                if ids.dtype != torch.int64 or ids.device != d or ids.numel() not in (1, n):
+                    raise ValueError("rows must be an int, or an int64 tensor of one id or %d ids on the "
+                                     "engine's device" % n)
+                ids = ids.reshape(-1).contiguous()
             _lib.call("pss_gather_dropout", self._h, ctypes.c_void_p(data.data_ptr()), DTYPES[data.dtype],
                       row_bytes // data.element_size(), ctypes.c_void_p(base_rows.data_ptr()),
-                      ctypes.c_void_p(fpos.data_ptr()), ctypes.c_void_p(off.data_ptr()), n, _p(p),
+                      ctypes.c_void_p(fpos.data_ptr()), ctypes.c_void_p(off.data_ptr()), n, float(p),
                       int(key) & 0xFFFFFFFFFFFFFFFF, row0, None if ids is None else ids.data_ptr(),
                       0 if ids is None else ids.numel(), ctypes.c_void_p(out.data_ptr()), _stream_ptr(stream, d))
             return out

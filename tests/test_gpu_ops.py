@@ -558,7 +558,7 @@ def test_gpu_refusals():
         ops.combine(y, r, residual=x.half())
     with pytest.raises(TypeError, match="device"):
         ops.dropout(x, 0.1, 0, rows=torch.zeros(1, dtype=torch.int64))
-    with pytest.raises(RuntimeError, match="differentiable|once"):
+    with pytest.raises(RuntimeError, match="differentiated again"):
         xg = x.clone().requires_grad_()
         g, = torch.autograd.grad(ops.dropout(xg, 0.5, 1).square().sum(), xg, create_graph=True)
         g.sum().backward()

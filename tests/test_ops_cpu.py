@@ -183,10 +183,13 @@ def test_refusals():
         ops.dropout(torch.tensor(1.0), 0.1, 0)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.route(x, 2)
-    with pytest.raises(ValueError, match="GPU"):
-        ops.dispatch(x, None)
-    with pytest.raises(ValueError, match="GPU"):
-        ops.combine(x, None)
+    i = torch.zeros(4, 2, dtype=torch.int32)
+    r = ops.Routing(i, torch.zeros(4, 2), torch.zeros(9, dtype=torch.int32), i, i.reshape(-1))
+    for f in (ops.dispatch, ops.combine):
+        with pytest.raises(TypeError, match="Routing"):
+            f(x, None)
+        with pytest.raises(ValueError, match="GPU"):
+            f(x, r)
 
 
 def _route_rc(tokens=0, experts=8, k=2, dtype=0, score=0, groups=1, top_groups=1, group_sum=1, scale=1.0, ld=8,
