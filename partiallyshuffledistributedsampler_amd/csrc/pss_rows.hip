@@ -184,13 +184,29 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// N logits of row t from expert e0 on, -inf past the last
+// N <= E logits of row t from expert e0 on, -inf past the last.  A lane whose values run past the end
+// reads the row's last N and shifts them down: no branch, no loads one by one.
+template <typename T, int N>
+__device__ __forceinline__ void load_end(const T *row, int e0, int E, float (&l)[N]) {
+    const int left = E - e0;
+    load(row + (left >= N ? e0 : left > 0 ? E - N : 0), N, l);
+    if (E % N) {
+        const int by = left >= N ? 0 : N - left;
+#pragma unroll
+        for (int s = 1; s < N; s *= 2)
+#pragma unroll
+            for (int i = 0; i < N; i++) l[i] = !(by & s) ? l[i] : i + s < N ? l[i + s] : -INFINITY;
+    }
+    if (left <= 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) l[i] = -INFINITY;
+}
 template <int N>
 __device__ __forceinline__ void load_logits(const RouteArgs &a, int64_t t, int e0, float (&l)[N]) {
-    const int64_t i = t * a.ld + e0;
-    if (a.dtype == 0) load((const float *)a.logits + i, a.E - e0, l, -INFINITY);
-    else if (a.dtype == 1) load((const __bf16 *)a.logits + i, a.E - e0, l, -INFINITY);
-    else load((const _Float16 *)a.logits + i, a.E - e0, l, -INFINITY);
+    const int64_t i = t * a.ld;
+    if (a.dtype == 0) load_end((const float *)a.logits + i, e0, a.E, l);
+    else if (a.dtype == 1) load_end((const __bf16 *)a.logits + i, e0, a.E, l);
+    else load_end((const _Float16 *)a.logits + i, e0, a.E, l);
 }
 __device__ __forceinline__ float one_logit(const RouteArgs &a, int64_t t, int e) {
     const int64_t i = t * a.ld + e;
@@ -215,9 +231,16 @@ template <int N> __device__ __forceinline__ void bitonic(uint32_t *x) {   // a b
         for (int i = 0; i < N; i++)
             if (!(i & h)) order2(x[i], x[i + h]);
 }
-// x[0, N) any -> falling (bitonic network)
+// x[0, N) any -> falling: bitonic, and for 8 the network of 19 comparisons (the fewest)
 template <int N> __device__ __forceinline__ void sort_falling(uint32_t *x) {
-    if constexpr (N > 1) {
+    if constexpr (N == 8) {
+        order2(x[0], x[2]); order2(x[1], x[3]); order2(x[4], x[6]); order2(x[5], x[7]);
+        order2(x[0], x[4]); order2(x[1], x[5]); order2(x[2], x[6]); order2(x[3], x[7]);
+        order2(x[0], x[1]); order2(x[2], x[3]); order2(x[4], x[5]); order2(x[6], x[7]);
+        order2(x[2], x[4]); order2(x[3], x[5]);
+        order2(x[1], x[4]); order2(x[3], x[6]);
+        order2(x[1], x[2]); order2(x[3], x[4]); order2(x[5], x[6]);
+    } else if constexpr (N > 1) {
         sort_falling<N / 2>(x);
         sort_falling<N / 2>(x + N / 2);
         // two falling halves: the larger of each mirrored pair first
@@ -282,35 +305,35 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return std::max(std::max(a, b), std::max(c, d));
 }
 
-// Choice value of a live logit in 64 bits (m, sum: the row's softmax statistics).
-__device__ __forceinline__ double choice64(const RouteArgs &a, bool by_logit, float l, int e, float m, double sum) {
-    double x = (double)l;
-    if (!by_logit) {
-        x = a.score == 0 ? exp(x - (double)m) / sum : 1.0 / (1.0 + exp(-x));
-        if (a.bias) x += (double)a.bias[e];
-    }
-    return x >= kLast ? x : kLast;
-}
-
 // The choice of a row's experts from values in 64 bits, one at a time, by a whole wave: lane j's expert.
 // It is the definition of the choice, and what the 32-bit choice leaves to it where its values are too
-// close to tell the order, too far from the best, or no numbers.  value: E + G doubles of LDS (groups).
-template <int V>
-__device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, int lane, const float (&l)[V], float m,
-                                        double sum, double *value) {
+// close to tell the order, too far from the best, or no numbers.  value: E + G doubles of LDS, in which
+// the row's logits stand; m: their maximum; sum: of their exponentials, set here if `exps`.
+// Kept as loops: the code is cold, and fetching it unrolled took longer than running it.
+__device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool exps, int lane, float m, double &sum,
+                                        double *value) {
     const int E = a.E, G = a.groups, S = E / G;
-    double c[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int e = lane * V + v;
-        c[v] = e < E && l[v] != -INFINITY ? choice64(a, by_logit, l[v], e, m, sum) : kDead;
+    sum = 1.0;
+    if (exps) {
+        sum = 0.0;
+#pragma unroll 1
+        for (int e = lane; e < E; e += 64) sum += value[e] == kDead ? 0.0 : exp(value[e] - (double)m);
+        sum = seg_reduce<64>(sum, Sum());
     }
+#pragma unroll 1
+    for (int e = lane; e < E; e += 64) {
+        double x = value[e];
+        if (x == kDead) continue;
+        if (!by_logit) {
+            const double t = exp(a.score == 0 ? x - (double)m : -x);
+            x = a.score == 0 ? t / sum : 1.0 / (1.0 + t);
+            if (a.bias) x += (double)a.bias[e];
+        }
+        value[e] = x >= kLast ? x : kLast;
+    }
+    wave_lds_sync();
     if (G > 1) {
         double *score = value + E;
-#pragma unroll
-        for (int v = 0; v < V; v++)
-            if (lane * V + v < E) value[lane * V + v] = c[v];
-        wave_lds_sync();
         double mine = kDead;
         if (lane < G) {
             double b2 = kDead;
@@ -330,39 +353,55 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, int l
             const double x = score[o];
             before += x > mine || (x == mine && o < lane);
         }
-        const uint64_t kept = __ballot(lane < G && before < a.top_groups);
+        if (lane < G && before >= a.top_groups)
+#pragma unroll 1
+            for (int s = 0; s < S; s++) value[lane * S + s] = kDead;
         wave_lds_sync();
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            const int e = lane * V + v;
-            if (e < E && !((kept >> (e / S)) & 1)) c[v] = kDead;
-        }
     }
     int my_e = -1;
     for (int j = 0; j < a.k; j++) {
         double best = kDead;
-        int be = -1;
-#pragma unroll
-        for (int v = 0; v < V; v++)
-            if (c[v] > best) { best = c[v]; be = lane * V + v; }
-        // the wave's maximum as ordered bits, high word first; of equal values the lowest lane's
+        int be = 1 << 20;
+#pragma unroll 4
+        for (int e = lane; e < E; e += 64) {
+            const double x = value[e];
+            be = x > best ? e : be;
+            best = x > best ? x : best;
+        }
+        // the wave's maximum as ordered bits, high word first; of equal values the lowest expert
         uint64_t u;
         best += 0.0;            // -0 is 0
         __builtin_memcpy(&u, &best, 8);
         u ^= (uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull;
         const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u, top = wave_max(hi);
-        uint64_t who = __ballot(hi == top);
+        bool on = hi == top;
+        uint64_t who = __ballot(on);
         if (who & (who - 1)) {
-            const uint32_t low = wave_max(hi == top ? lo : 0u);
-            who = __ballot(hi == top && lo == low);
+            const uint32_t low = wave_max(on ? lo : 0u);
+            on = on && lo == low;
+            who = __ballot(on);
         }
-        const int won = __builtin_amdgcn_readlane(be, __builtin_ctzll(who));    // -1: none is left
-        if (lane == j) my_e = won;
-#pragma unroll
-        for (int v = 0; v < V; v++)
-            if (lane * V + v == won) c[v] = kDead;
+        int won = __builtin_amdgcn_readlane(be, __builtin_ctzll(who));
+        if (who & (who - 1)) won = (int)~wave_max(on ? ~(uint32_t)be : 0u);
+        const bool any = won < E;
+        if (lane == j) my_e = any ? won : -1;
+        if (any && lane == 0) value[won] = kDead;
+        wave_lds_sync();
     }
     return my_e;
+}
+
+// A group's value as an unsigned key of its order, the lowest 6 bits the index (lower first); and back,
+// to within those bits.  -0 is 0.
+__device__ __forceinline__ uint32_t group_key(float x, uint32_t g) {
+    uint32_t u = __float_as_uint(x + 0.f);
+    u ^= (uint32_t)((int32_t)u >> 31) | 0x80000000u;
+    return (u & ~63u) | (63u - g);
+}
+__device__ __forceinline__ float group_value(uint32_t key) {
+    uint32_t u = key & ~63u;
+    u ^= u & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu;
+    return __uint_as_float(u);
 }
 
 constexpr int kRouteThreads = 512;
@@ -445,7 +484,7 @@ __device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i,
 // nearer than the keys' and the scores' error is left to choose64 after the others.
 template <int L, int V, int KP>
 __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
-    extern __shared__ uint64_t lds[];
+    extern __shared__ __align__(16) uint64_t lds[];
     __shared__ uint32_t scan_tmp[kRouteThreads / 64], first[64];
     __shared__ unsigned long long odd_rows;
     constexpr int kIndex = L * V <= 256 ? 8 : 10;
@@ -454,9 +493,10 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     int lane = threadIdx.x & (L - 1);
     const int seg = threadIdx.x / L;
     uint64_t *mask = lds;                                                  // [E]
-    double *room = (double *)(mask + E);                                   // groups alone:
-    float *score = (float *)room + (size_t)seg * G;                        // [segments][G]
-    float *value = (float *)room + (size_t)(kRouteThreads / L) * G + (size_t)seg * (L * V);  // [segments][L * V]
+    double *room = (double *)(mask + (E + 1) / 2 * 2);                     // 16-byte aligned; groups alone:
+    const int Gp = (G + 3) & ~3;
+    uint32_t *score = (uint32_t *)room + (size_t)seg * Gp;                 // [segments][Gp], the last ones 0
+    float *value = (float *)room + (size_t)(kRouteThreads / L) * Gp + (size_t)seg * (L * V);  // [segments][L * V]
     const int64_t t0 = (int64_t)blockIdx.x * kRouteChunk;
     const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
     const bool by_logit = !a.bias && (G == 1 || a.group_sum == 1);
@@ -464,6 +504,8 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     const bool exps = a.score == 0 && !(by_logit && a.renorm);             // softmax statistics wanted
     const uint32_t inv = ((1u << 20) + S - 1) / S;                         // e / S = e * inv >> 20, e < 1024
     for (int i = threadIdx.x; i < E; i += kRouteThreads) mask[i] = 0;
+    if (G > 1)
+        for (int i = threadIdx.x; i < kRouteThreads / L * Gp; i += kRouteThreads) ((uint32_t *)room)[i] = 0;
     if (threadIdx.x == 0) odd_rows = 0;
     // (in LDS, value v of lane x at v / 4 * 4 * L + 4 * x + v % 4: registers are what limits the waves)
     __shared__ float bias[L * V < 64 ? 64 : L * V];
@@ -484,15 +526,15 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         const bool row = i < nt;
         const int64_t t = t0 + (row ? i : 0);
         const bool on = row && (!a.valid || a.valid[t]);
-        // c: -inf where the expert is masked
+        // c: a NaN or -inf where the expert is masked (0 * l is a NaN for l = -inf; the maxima below
+        // leave a NaN out, and its key is 0).  A row that has a NaN or +inf is left to choose64.
         float c[V];
         load_logits(a, t, lane * V, c);
-        bool nan = false;
+        bool odd = false;
         float m = -INFINITY, sum = 1.f, eps = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; v++) nan |= c[v] != c[v];
-        nan = seg_reduce<L>((int)nan, Or()) != 0;
-        if (a.score == 0 && (exps || !by_logit)) {
+        for (int v = 0; v < V; v++) odd |= __builtin_amdgcn_classf(c[v], 0x203);
+        if (exps) {
 #pragma unroll
             for (int v = 0; v < V; v++) m = fmaxf(m, c[v]);
             m = seg_max<L>(m);
@@ -510,24 +552,25 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                 eps = 2e-6f;
                 const float r = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
-                for (int v = 0; v < V; v++) c[v] = c[v] == -INFINITY ? c[v] : s[v] * r;
+                for (int v = 0; v < V; v++) c[v] = fmaf(c[v], 0.f, s[v] * r);
                 if (a.bias) add_bias(c);
             }
         } else if (!by_logit) {
             // off by 5e-7: the exponent's rounding times s (1 - s), and a unit each of exp, sum, reciprocal
             eps = 5e-7f;
 #pragma unroll
-            for (int v = 0; v < V; v++)
-                c[v] = c[v] == -INFINITY ? c[v] : __builtin_amdgcn_rcpf(1.f + fast_exp(-c[v]));
+            for (int v = 0; v < V; v++) c[v] = fmaf(c[v], 0.f, __builtin_amdgcn_rcpf(1.f + fast_exp(-c[v])));
             if (a.bias) add_bias(c);
         }
-        bool odd = false;
         if (G > 1) {
+#pragma unroll
+            for (int v = 0; v < V; v++) c[v] = fmaxf(c[v], -INFINITY);      // (a median takes no NaN)
             // the two best of every group: a lane's values one by one, then across lanes, or through LDS
             if ((S & (S - 1)) == 0) {
                 float b1 = -INFINITY, b2 = -INFINITY;
-                auto flush = [&](int e) {       // of the group that ends with expert e
-                    score[((uint32_t)e * inv) >> 20] = a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+                auto flush = [&](int e) {       // of expert e's group
+                    const uint32_t g = ((uint32_t)e * inv) >> 20;
+                    score[g] = group_key(a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1, g);
                 };
 #pragma unroll
                 for (int v = 0; v < V; v++) {
@@ -562,37 +605,37 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                     float b1 = -INFINITY, b2 = -INFINITY;
                     for (int s = 0; s < S; s++) {
                         const float x = value[g * S + s];
-                        b2 = fmaxf(b2, fminf(b1, x));
+                        b2 = __builtin_amdgcn_fmed3f(b1, b2, x);
                         b1 = fmaxf(b1, x);
                     }
-                    score[g] = a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+                    score[g] = group_key(a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1, g);
                 }
             }
             wave_lds_sync();
+            // a group is kept if fewer than top_groups keys are larger
             uint64_t kept = 0;
-            float least = INFINITY, most = -INFINITY;     // of the groups kept, and of the others
+            uint32_t least = 0xFFFFFFFFu, most = 0;       // of the groups kept, and of the others
             for (int g = lane; g < G; g += L) {
-                const float x = score[g];
+                const uint32_t x = score[g];
                 int before = 0;
-#pragma unroll 4
-                for (int o = 0; o < G; o++) {
-                    const float y = score[o];
-                    before += y > x || (y == x && o < g);
+                for (int o = 0; o < G; o += 4) {
+                    const uint4 y = *(const uint4 *)(score + o);
+                    before += (y.x > x) + (y.y > x) + (y.z > x) + (y.w > x);
                 }
                 if (before < a.top_groups) {
                     kept |= 1ull << g;
-                    least = fminf(least, x);
+                    least = std::min(least, x);
                 } else {
-                    most = fmaxf(most, x);
+                    most = std::max(most, x);
                 }
             }
             kept = seg_reduce<L>(kept, Or());
-            if (!by_logit) {
-                least = seg_min<L>(least);
-                most = seg_max<L>(most);
-                // two scores' errors on either side, and the roundings of their sums
-                odd = most > -INFINITY &&
-                      !(least - most > 4.f * eps + 8.f * 0x1p-24f * fmaxf(fabsf(least), fabsf(most)));
+            if (!exact) {
+                least = seg_reduce<L>(least, Min());
+                most = seg_reduce<L>(most, Max());
+                // two scores' errors on either side, the roundings of their sums, and the keys' 64 units
+                const float p = group_value(least), q = group_value(most);
+                if (most) odd |= !(p - q > 4.f * eps + 0x1p-17f * fmaxf(fabsf(p), fabsf(q))) && q > -INFINITY;
             }
             wave_lds_sync();
             const uint32_t g0 = ((uint32_t)(lane * V) * inv) >> 20;
@@ -623,13 +666,15 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
             top = seg_max<L>(top);
             // scores span less than 2 unless a bias does more; values at or below the floor have key 0
             // and, where one of them is chosen, choose64 tells them apart and from masked ones
+            // (the conversion makes 0 of what is negative, and of a NaN)
             constexpr float kSteps = (float)((1 << (32 - kIndex)) - 8);
             const float scale = by_logit ? kSteps / 16.f : kSteps / 2.f;
             odd |= !(fabsf(top) < 1e6f) && top > -INFINITY;
             eps = 2.f * scale * (eps > 0.f ? eps + 0x1p-23f * fmaxf(fabsf(top), 1.f) : 0.f) + 4.f;
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const uint32_t q = (uint32_t)fmaxf(fmaf(c[v] - top, scale, kSteps), 0.f);
+                uint32_t q;
+                asm("v_cvt_u32_f32 %0, %1" : "=v"(q) : "v"(fmaf(c[v] - top, scale, kSteps)));
                 key[v] = q << kIndex | (kIndexMask - v);
             }
         }
@@ -641,7 +686,6 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         int my_e;
         if (exact) {
             my_e = mine ? (int)(kExactMask - (mine & kExactMask)) : -1;
-            odd = nan;
         } else {
             my_e = (int)(kIndexMask - (mine & kIndexMask));
             // neighbours nearer than eps, or one at the floor; then the best key that was not chosen
@@ -664,43 +708,36 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
             }
             rest = seg_reduce<L>(rest, Max());
             odd |= (float)((last >> kIndex) - (rest >> kIndex)) < eps;
-            odd |= nan;
         }
-        odd = odd && on;
-        if (!on || lane >= k) my_e = -1;
+        odd = seg_reduce<L>((int)odd, Or()) != 0 && on;
+        if (!on || odd || lane >= k) my_e = -1;     // (a key at the floor may be of no expert at all)
         if (odd && lane == 0) atomicOr(&odd_rows, 1ull << i);
-        finish_row<L>(a, t, i, row && !odd, lane, my_e, nan, m, sum, mask);
+        finish_row<L>(a, t, i, row && !odd, lane, my_e, false, m, sum, mask);
     }
     __syncthreads();
     // the rows left, a wave each
-    constexpr int VX = L == 64 ? V : (V + 3) / 4;
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
     const int odds = __popcll(odd_rows);
+    double *row64 = room + (size_t)wave * (E + G);
     for (int n0 = wave; n0 < odds; n0 += kRouteThreads / 64) {
         unsigned long long left = odd_rows;
         for (int n = 0; n < n0; n++) left &= left - 1;
         const int i = __ffsll(left) - 1;
         const int64_t t = t0 + i;
-        float l[VX];
-        load_logits(a, t, wl * VX, l);
         bool nan = false;
         float m = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < VX; v++) {
-            nan |= l[v] != l[v];
-            m = fmaxf(m, l[v]);
+#pragma unroll 4
+        for (int e = wl; e < E; e += 64) {
+            const float x = one_logit(a, t, e);
+            nan |= x != x;
+            m = fmaxf(m, x);
+            row64[e] = (double)x;
         }
-        nan = seg_reduce<64>((int)nan, Or()) != 0;
+        nan = __any(nan);
         m = seg_max<64>(m);
-        double sum = 1.0;
-        if (exps) {
-            sum = 0.0;
-#pragma unroll
-            for (int v = 0; v < VX; v++)
-                if (l[v] != -INFINITY) sum += exp((double)l[v] - (double)m);
-            sum = seg_reduce<64>(sum, Sum());
-        }
-        const int my_e = choose64<VX>(a, by_logit, wl, l, m, sum, room + (size_t)wave * (E + G));
+        wave_lds_sync();
+        double sum;
+        const int my_e = choose64(a, by_logit, exps, wl, m, sum, row64);
         finish_row<64>(a, t, i, true, wl, my_e, nan, m, (float)sum, mask);
     }
     __syncthreads();
@@ -756,7 +793,7 @@ __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict_
 // Places of one chunk's slots.
 __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
                                                                const int32_t *__restrict__ totals) {
-    extern __shared__ uint64_t lds[];
+    extern __shared__ __align__(16) uint64_t lds[];
     __shared__ uint64_t scan_tmp[kRouteThreads / 64];
     __shared__ uint32_t first[64];
     const int E = a.E;
@@ -796,7 +833,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
 template <typename T, int L, int V>
 __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const float *__restrict__ dweights,
                                                               T *__restrict__ dlogits) {
-    extern __shared__ uint64_t lds[];
+    extern __shared__ __align__(16) uint64_t lds[];
     const int E = a.E, k = a.k;
     const int lane = threadIdx.x & (L - 1), seg = threadIdx.x / L;
     float *d = (float *)lds + (size_t)seg * (L * V);
@@ -1100,26 +1137,26 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
 hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
     const int64_t chunks = route_chunks(a.T);
     const int S = a.E / a.groups;
+    hipError_t err = hipSuccess;
     by_width(a.E, [&](auto L, auto V) {
-        // masks; the bases (one chunk); with groups their scores and, for groups of no power of two, the
-        // values of every row at once, or the values and scores in 64 bits of a row for every wave
+        // masks; the bases (one chunk); the groups' keys and, for groups of no power of two, the values of
+        // every row at once; or a row's values and its groups' in 64 bits for every wave
         const size_t rows = kRouteThreads / decltype(L)::value, E = a.E, G = a.groups;
-        size_t room = 4 * E;
-        if (G > 1) {
-            room = std::max(room, rows * 4 * (G + (S & (S - 1) ? (size_t)(L * V) : 0)));
-            room = std::max(room, kRouteThreads / 64 * 8 * (E + G));
-        }
-        const size_t lds = 8 * E + room;
+        size_t room = std::max(4 * E, kRouteThreads / 64 * 8 * (E + G));
+        if (G > 1) room = std::max(room, rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
+        const size_t lds = 8 * ((E + 1) / 2 * 2) + room;
         auto go = [&](auto KP) {
-            hipLaunchKernelGGL((k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value>),
-                               dim3((unsigned)chunks), dim3(kRouteThreads), lds, s, a);
+            const auto kern = k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value>;
+            if (lds > 64 * 1024)
+                err = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (err == hipSuccess) hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kRouteThreads), lds, s, a);
         };
         if (a.k <= 4) go(std::integral_constant<int, 4>());
         else if (a.k <= 8) go(std::integral_constant<int, 8>());
         else go(std::integral_constant<int, 16>());
     });
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !a.mask) return e;
+    if (err == hipSuccess) err = hipGetLastError();
+    if (err != hipSuccess || !a.mask) return err;
     hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 7) / 8)), dim3(1024), 0, s, a.mask, a.before, a.totals,
                        chunks, a.E);
     hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads), 12 * (size_t)a.E, s, a, a.before,
