@@ -265,6 +265,7 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
  *   offsets[e] = rows of the experts before e, offsets[experts] = rows in all.  Slot s = t * k + j
  *   has the place pos[s] in the order by (expert, t); slots without an expert come after
  *   offsets[experts], in their own order; src is the inverse of pos.
+ *   slopes (NULL: not wanted) gets 1 - s of the chosen experts for the gradient of PSS_SIGMOID.
  * experts <= 1024, k <= 16, groups <= 64, tokens * k < 2^31.  ws: pss_route_workspace bytes, used by
  * this call alone while it runs.  Results do not depend on timing: no order of atomics enters. */
 #define PSS_SOFTMAX 0
@@ -272,13 +273,14 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
 int64_t pss_route_workspace(int64_t tokens, int32_t experts);
 int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype, int32_t score,
               const float *bias, const uint8_t *valid, int32_t groups, int32_t top_groups, int32_t group_sum,
-              int32_t renorm, double scale, int32_t *out_experts, float *out_weights, int32_t *offsets, int32_t *pos,
-              int32_t *src, void *ws, int64_t ws_bytes, void *stream);
+              int32_t renorm, double scale, int32_t *out_experts, float *out_weights, float *slopes, int32_t *offsets,
+              int32_t *pos, int32_t *src, void *ws, int64_t ws_bytes, void *stream);
 /* The weights' gradient dweights [tokens, k] -> dlogits [tokens, experts] (contiguous, every value
- * written); logits, chosen and weights as pss_route had and gave them. */
+ * written); chosen, weights and (PSS_SIGMOID) slopes as pss_route gave them, logits as it had them
+ * (read for PSS_SOFTMAX without renorm alone, else NULL will do). */
 int pss_route_grad(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype,
                    int32_t score, int32_t renorm, double scale, const int32_t *chosen, const float *weights,
-                   const float *dweights, void *dlogits, void *stream);
+                   const float *slopes, const float *dweights, void *dlogits, void *stream);
 
 /* Rows into expert order: xs[pos[t, j]] = x[t]; 0 where the slot has no expert. */
 int pss_dispatch(const void *x, int64_t ldx, int64_t tokens, int32_t k, int64_t cols, int32_t dtype,

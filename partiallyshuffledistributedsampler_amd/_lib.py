@@ -63,9 +63,9 @@ SIGNATURES = {
                             _vp, _vp], ctypes.c_int),
     "pss_route_workspace": ([_i64, _i32], _i64),
     "pss_route": ([_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f64,
-                   _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp], ctypes.c_int),
+                   _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp], ctypes.c_int),
     "pss_route_grad": ([_vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f64, _vp, _vp, _vp, _vp,
-                        _vp], ctypes.c_int),
+                        _vp, _vp], ctypes.c_int),
     "pss_dispatch": ([_vp, _i64, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp], ctypes.c_int),
     "pss_combine": ([_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _f64, _u64, _i64, _vp,
                      _i64, _vp, _vp], ctypes.c_int),

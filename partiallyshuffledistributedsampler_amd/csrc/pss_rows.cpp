@@ -186,8 +186,8 @@ int64_t pss_route_workspace(int64_t tokens, int32_t experts) {
 
 int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype, int32_t score,
               const float *bias, const uint8_t *valid, int32_t groups, int32_t top_groups, int32_t group_sum,
-              int32_t renorm, double scale, int32_t *out_experts, float *out_weights, int32_t *offsets, int32_t *pos,
-              int32_t *src, void *ws, int64_t ws_bytes, void *stream) {
+              int32_t renorm, double scale, int32_t *out_experts, float *out_weights, float *slopes, int32_t *offsets,
+              int32_t *pos, int32_t *src, void *ws, int64_t ws_bytes, void *stream) {
     RouteArgs a;
     const int rc = route_args(&a, logits, ld, tokens, experts, k, dtype, score, renorm, scale);
     if (rc) return rc;
@@ -209,6 +209,7 @@ int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, i
     a.group_sum = group_sum;
     a.experts = out_experts;
     a.weights = out_weights;
+    a.slopes = score == PSS_SIGMOID ? slopes : nullptr;
     a.offsets = offsets;
     a.pos = pos;
     a.src = src;
@@ -224,11 +225,15 @@ int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, i
 
 int pss_route_grad(const void *logits, int64_t ld, int64_t tokens, int32_t experts, int32_t k, int32_t dtype,
                    int32_t score, int32_t renorm, double scale, const int32_t *chosen, const float *weights,
-                   const float *dweights, void *dlogits, void *stream) {
+                   const float *slopes, const float *dweights, void *dlogits, void *stream) {
     RouteArgs a;
-    const int rc = route_args(&a, logits, ld, tokens, experts, k, dtype, score, renorm, scale);
+    // the logits are read for a softmax that was not renormalised alone
+    const bool full = score == PSS_SOFTMAX && !renorm;
+    const int rc = route_args(&a, full ? logits : dlogits, ld, tokens, experts, k, dtype, score, renorm, scale);
     if (rc) return rc;
-    if (tokens > 0 && (!chosen || !weights || !dweights || !dlogits)) return set_error(PSS_EINVAL, "route_grad: NULL argument");
+    if (tokens > 0 && (!chosen || !weights || !dweights || !dlogits || (score == PSS_SIGMOID && !slopes)))
+        return set_error(PSS_EINVAL, "route_grad: NULL argument");
+    a.slopes = const_cast<float *>(slopes);
     a.experts = const_cast<int32_t *>(chosen);
     a.weights = const_cast<float *>(weights);
     ROWS_HIP(launch_route_grad(a, dweights, dlogits, (hipStream_t)stream));

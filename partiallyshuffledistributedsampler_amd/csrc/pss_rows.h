@@ -43,6 +43,7 @@ struct RouteArgs {
     int32_t groups, top_groups, group_sum;
     int32_t *experts;       // [T, k]
     float *weights;         // [T, k]
+    float *slopes;          // [T, k] 1 - sigmoid of the chosen, or NULL
     int32_t *offsets;       // [E + 1]
     int32_t *pos, *src;     // [T * k]
     // workspace (NULL with one chunk): rows of each chunk and expert, rows before, rows in all
@@ -54,7 +55,8 @@ constexpr int kRouteChunk = 64;     // rows of a workgroup: one bit of a 64-bit 
 constexpr int kRouteMaxE = 1024, kRouteMaxK = 16, kRouteMaxGroups = 64;
 static inline int64_t route_chunks(int64_t T) { return T <= kRouteChunk ? 1 : (T + kRouteChunk - 1) / kRouteChunk; }
 hipError_t launch_route(const RouteArgs &a, hipStream_t s);
-// dweights [T, k] -> dlogits [T, E] (contiguous); reads logits, experts, weights of `a`
+// dweights [T, k] -> dlogits [T, E] (contiguous); reads experts, weights, slopes (sigmoid) or logits
+// (softmax not renormalised) of `a`
 hipError_t launch_route_grad(const RouteArgs &a, const float *dweights, void *dlogits, hipStream_t s);
 
 struct MoveArgs {           // rows between their own order (T) and the experts' (T * k)

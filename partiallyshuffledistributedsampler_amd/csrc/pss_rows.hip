@@ -423,25 +423,38 @@ __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tm
 
 // Places of the slots of one chunk of 64 rows: rows of an expert in the order of the rows (mask[e]: the
 // chunk's rows that have it, base[e]: where its rows of this chunk begin), slots without an expert from
-// unused0 on.  All threads; `first` holds 64 words.
+// unused0 on.  All threads, at most two slots each; `first` holds 64 words.
+static_assert(kRouteChunk * kRouteMaxK <= 2 * kRouteThreads, "slots of a chunk");
 __device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int nt, const uint64_t *mask,
                                             const int32_t *base, int32_t unused0, uint32_t *first) {
-    const int k = a.k;
-    if (threadIdx.x < 64) {     // slots without an expert in the rows before
-        const int t = threadIdx.x;
-        uint32_t un = 0;
-        if (t < nt)
-            for (int j = 0; j < k; j++) un += a.experts[(t0 + t) * k + j] < 0;
-        const uint32_t incl = wave_incl_scan(un);
-        first[t] = incl - un - (k - un);        // + j = the slot's rank: they are a row's last slots
+    const int k = a.k, n = nt * k;
+    int e[2];
+    bool none = false;
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int i = threadIdx.x + q * kRouteThreads;
+        e[q] = i < n ? a.experts[t0 * k + i] : 0;
+        none |= e[q] < 0;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt * k; i += blockDim.x) {
+    if (__syncthreads_or(none)) {
+        if (threadIdx.x < 64) {     // slots without an expert in the rows before
+            const int t = threadIdx.x;
+            uint32_t un = 0;
+            if (t < nt)
+                for (int j = 0; j < k; j++) un += a.experts[(t0 + t) * k + j] < 0;
+            const uint32_t incl = wave_incl_scan(un);
+            first[t] = incl - un - (k - un);        // + j = the slot's rank: they are a row's last slots
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int i = threadIdx.x + q * kRouteThreads;
+        if (i >= n) break;
         const int t = i / k, j = i - t * k;
         const int64_t slot = t0 * k + i;
-        const int e = a.experts[slot];
-        const int32_t p = e < 0 ? unused0 + (int32_t)(first[t] + j)
-                                : base[e] + __popcll(mask[e] & ((1ull << t) - 1));
+        const int32_t p = e[q] < 0 ? unused0 + (int32_t)(first[t] + j)
+                                   : base[e[q]] + __popcll(mask[e[q]] & ((1ull << t) - 1));
         a.pos[slot] = p;
         a.src[p] = (int32_t)slot;
     }
@@ -472,6 +485,8 @@ __device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i,
     if (write && lane < a.k) {
         a.experts[t * a.k + lane] = my_e;
         a.weights[t * a.k + lane] = w;
+        // 1 - sigmoid, for the gradient: its rows would else be read again for k values each
+        if (a.slopes) a.slopes[t * a.k + lane] = used ? 1.f / (1.f + fast_exp(lw)) : 0.f;
         if (my_e >= 0) atomicOr((unsigned long long *)&mask[my_e], 1ull << i);
     }
 }
@@ -790,7 +805,7 @@ __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict_
     }
 }
 
-// Places of one chunk's slots.
+// Places of one chunk's slots.  Without the sums of k_route_scan a workgroup counts all chunks itself.
 __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
                                                                const int32_t *__restrict__ totals) {
     extern __shared__ __align__(16) uint64_t lds[];
@@ -808,8 +823,17 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
         uint32_t all = 0, prev = 0;
         if (e < E) {
             mask[e] = a.mask[c * E + e];
-            all = (uint32_t)totals[e];
-            prev = (uint32_t)before[c * E + e];
+            if (before) {
+                all = (uint32_t)totals[e];
+                prev = (uint32_t)before[c * E + e];
+            } else {
+#pragma unroll 8
+                for (int64_t b = 0; b < gridDim.x; b++) {
+                    const uint32_t n = __popcll(a.mask[b * E + e]);
+                    all += n;
+                    prev += b < c ? n : 0u;
+                }
+            }
         }
         uint64_t sum;
         const uint64_t pre = run + block_excl_scan<kRouteThreads>((uint64_t)prev << 32 | all, scan_tmp, sum);
@@ -852,7 +876,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const
         }
         const float dot = seg_reduce<L>(g * w, Sum());
         float x = w * (a.renorm ? g - dot / a.scale : g);
-        if (a.score == 1 && e >= 0) x /= 1.f + expf(Value<T>::up(lp[e]));
+        if (a.score == 1 && e >= 0) x *= a.slopes[tt * k + lane];
 #pragma unroll
         for (int v = 0; v < V; v++) d[v * L + lane] = 0.f;
         wave_lds_sync();
@@ -1157,10 +1181,14 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
     });
     if (err == hipSuccess) err = hipGetLastError();
     if (err != hipSuccess || !a.mask) return err;
-    hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 7) / 8)), dim3(1024), 0, s, a.mask, a.before, a.totals,
-                       chunks, a.E);
-    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads), 12 * (size_t)a.E, s, a, a.before,
-                       a.totals);
+    // few chunks: every workgroup of the last kernel sums them, one launch less
+    // (a call with 2048 rows and 64 experts 11.4 us, with 2049 rows 14.1)
+    const bool sums = chunks > 32;
+    if (sums)
+        hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 7) / 8)), dim3(1024), 0, s, a.mask, a.before, a.totals,
+                           chunks, a.E);
+    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads), 12 * (size_t)a.E, s, a,
+                       sums ? a.before : nullptr, a.totals);
     return hipGetLastError();
 }
 

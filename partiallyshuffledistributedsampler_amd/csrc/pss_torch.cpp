@@ -180,35 +180,44 @@ struct Route : torch::autograd::Function<Route> {
         Tensor experts = at::empty({r.n, k}, i32), weights = at::empty({r.n, k}, logits.options().dtype(at::kFloat));
         Tensor offsets = at::empty({r.d + 1}, i32), pos = at::empty({r.n, k}, i32), src = at::empty({r.n * k}, i32);
         const int64_t need = lib.pss_route_workspace(r.n, (int32_t)r.d);
-        Tensor ws;
+        Tensor ws, slopes;
         if (need) ws = at::empty({need}, logits.options().dtype(at::kByte));
+        const bool grad = logits.requires_grad();
+        if (grad && score == PSS_SIGMOID) slopes = at::empty({r.n, k}, weights.options());
         check(lib.pss_route(r.t.const_data_ptr(), r.ld, r.n, (int32_t)r.d, (int32_t)k, dtype_of(logits), (int32_t)score,
-                            (const float *)ptr(get(bias)), (const uint8_t *)ptr(get(valid)), (int32_t)groups, (int32_t)top_groups,
-                            (int32_t)group_sum, renorm, scale, experts.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                            (const float *)ptr(get(bias)), (const uint8_t *)ptr(get(valid)), (int32_t)groups,
+                            (int32_t)top_groups, (int32_t)group_sum, renorm, scale, experts.data_ptr<int32_t>(),
+                            weights.data_ptr<float>(), slopes.defined() ? slopes.data_ptr<float>() : nullptr,
                             offsets.data_ptr<int32_t>(), pos.data_ptr<int32_t>(), src.data_ptr<int32_t>(),
                             need ? ws.data_ptr() : nullptr, need, stream_of(logits)),
               "pss_route");
-        ctx->saved_data["score"] = score;
-        ctx->saved_data["renorm"] = renorm;
-        ctx->saved_data["scale"] = scale;
         ctx->mark_non_differentiable({experts, offsets, pos, src});
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({logits, experts, weights});
+        if (grad) {
+            ctx->saved_data["score"] = score;
+            ctx->saved_data["renorm"] = renorm;
+            ctx->saved_data["scale"] = scale;
+            ctx->saved_data["experts"] = r.d;
+            ctx->saved_data["dtype"] = (int64_t)logits.scalar_type();
+            ctx->save_for_backward({score == PSS_SOFTMAX && !renorm ? logits : Tensor(), experts, weights, slopes});
+        }
         return {experts, weights, offsets, pos, src};
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
         variable_list out(10);
         if (!g[1].defined() || !ctx->needs_input_grad(0)) return out;
         const auto saved = ctx->get_saved_variables();
-        const Rows r(saved[0]);
+        const Tensor &experts = saved[1], &weights = saved[2], &slopes = saved[3];
+        const int64_t n = experts.size(0), k = experts.size(1), e = ctx->saved_data["experts"].toInt();
         const Tensor dw = g[1].contiguous();
-        c10::DeviceGuard guard(r.t.device());
-        out[0] = at::empty({r.n, r.d}, r.t.options());
-        check(lib.pss_route_grad(r.t.const_data_ptr(), r.ld, r.n, (int32_t)r.d, (int32_t)saved[1].size(1), dtype_of(r.t),
+        c10::DeviceGuard guard(dw.device());
+        out[0] = at::empty({n, e}, weights.options().dtype((at::ScalarType)ctx->saved_data["dtype"].toInt()));
+        const Rows r(saved[0].defined() ? saved[0] : out[0]);
+        check(lib.pss_route_grad(r.t.const_data_ptr(), r.ld, n, (int32_t)e, (int32_t)k, dtype_of(out[0]),
                                  (int32_t)ctx->saved_data["score"].toInt(), ctx->saved_data["renorm"].toBool(),
-                                 ctx->saved_data["scale"].toDouble(), saved[1].const_data_ptr<int32_t>(),
-                                 saved[2].const_data_ptr<float>(), dw.const_data_ptr<float>(), out[0].data_ptr(),
-                                 stream_of(r.t)),
+                                 ctx->saved_data["scale"].toDouble(), experts.const_data_ptr<int32_t>(),
+                                 weights.const_data_ptr<float>(), (const float *)ptr(slopes),
+                                 dw.const_data_ptr<float>(), out[0].data_ptr(), stream_of(dw)),
               "pss_route_grad");
         return once(g, std::move(out));
     }

@@ -7,6 +7,7 @@ GPU; BASELINE configs[0] runs there without a GPU).  A GPU engine never falls ba
 its device methods raise without a ROCm GPU.
 """
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -167,12 +168,15 @@ class IndexEngine:
         p > 0: the rows (float32, bfloat16 or float16) with dropout, in the same pass
         (pss_gather_dropout) -- exactly ops.dropout(rows flattened to [n, values], p, key, rows)."""
         d = self._dev()
-        fpos = fpos.reshape(-1).contiguous()
-        off = off.reshape(-1).to(torch.int32).contiguous()
-        base_rows = base_rows.to(device=d, dtype=torch.int64).contiguous()
+        if fpos.dim() != 1 or not fpos.is_contiguous():
+            fpos = fpos.reshape(-1).contiguous()
+        if off.dim() != 1 or off.dtype != torch.int32 or not off.is_contiguous():
+            off = off.reshape(-1).to(torch.int32).contiguous()
+        if base_rows.device != d or base_rows.dtype != torch.int64 or not base_rows.is_contiguous():
+            base_rows = base_rows.to(device=d, dtype=torch.int64).contiguous()
         assert data.device == d and data.is_contiguous() and fpos.device == d
         n = fpos.numel()
-        row_bytes = data[0].numel() * data.element_size() if data.dim() > 0 and data.shape[0] else 0
+        row_bytes = math.prod(data.shape[1:]) * data.element_size() if data.dim() > 0 and data.shape[0] else 0
         if out is None:
             out = torch.empty((n,) + tuple(data.shape[1:]), dtype=data.dtype, device=d)
         if p:
@@ -190,11 +194,10 @@ class IndexEngine:
                     raise ValueError("rows must be an int, or an int64 tensor of one id or %d ids on the "
                                      "engine's device" % n)
                 ids = ids.reshape(-1).contiguous()
-            _lib.call("pss_gather_dropout", self._h, ctypes.c_void_p(data.data_ptr()), DTYPES[data.dtype],
-                      row_bytes // data.element_size(), ctypes.c_void_p(base_rows.data_ptr()),
-                      ctypes.c_void_p(fpos.data_ptr()), ctypes.c_void_p(off.data_ptr()), n, float(p),
-                      int(key) & 0xFFFFFFFFFFFFFFFF, row0, None if ids is None else ids.data_ptr(),
-                      0 if ids is None else ids.numel(), ctypes.c_void_p(out.data_ptr()), _stream_ptr(stream, d))
+            _lib.call("pss_gather_dropout", self._h, data.data_ptr(), DTYPES[data.dtype],
+                      row_bytes // data.element_size(), base_rows.data_ptr(), fpos.data_ptr(), off.data_ptr(), n,
+                      float(p), int(key) & 0xFFFFFFFFFFFFFFFF, row0, None if ids is None else ids.data_ptr(),
+                      0 if ids is None else ids.numel(), out.data_ptr(), _stream_ptr(stream, d))
             return out
         _lib.call("pss_gather", self._h, ctypes.c_void_p(data.data_ptr()), row_bytes,
                   ctypes.c_void_p(base_rows.data_ptr()), ctypes.c_void_p(fpos.data_ptr()),

@@ -196,7 +196,7 @@ def _route_rc(tokens=0, experts=8, k=2, dtype=0, score=0, groups=1, top_groups=1
               logits=None, offsets=1):
     lib = _lib.load()
     return lib.pss_route(logits, ld, tokens, experts, k, dtype, score, None, None, groups, top_groups, group_sum, 1,
-                         scale, None, None, offsets, None, None, None, 0, None)
+                         scale, None, None, None, offsets, None, None, None, 0, None)
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -237,7 +237,9 @@ def test_other_entries_refuse_on_the_host():
     assert lib.pss_combine(None, 4, 2, 8, 0, None, None, None, None, 0, 0.0, 0, 0, None, 0, None, None) == 1
     assert lib.pss_combine(None, 0, 2, 8, 0, None, None, None, None, 0, 2.0, 0, 0, None, 0, None, None) == 1
     assert lib.pss_combine_grad(None, 8, None, 4, 2, 8, 0, None, None, None, 0.0, 0, 0, None, 0, None, None, None) == 1
-    assert lib.pss_route_grad(None, 8, 4, 8, 2, 0, 0, 1, 1.0, None, None, None, None, None) == 1
+    assert lib.pss_route_grad(None, 8, 4, 8, 2, 0, 0, 1, 1.0, None, None, None, None, None, None) == 1
+    # a sigmoid's gradient needs the slopes (nothing is read: the pointers are no addresses)
+    assert lib.pss_route_grad(None, 8, 4, 8, 2, 0, 1, 1, 1.0, 8, 8, None, 8, 8, None) == 1
     # handles: no sampler, no epoch
     assert lib.pss_gather_dropout(None, None, 0, 8, None, None, None, 0, 0.5, 0, 0, None, 0, None, None) == 1
     assert lib.pss_route_workspace(64, 64) == 0 and lib.pss_route_workspace(65, 64) > 0
