@@ -307,37 +307,59 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 
 // The choice of a row's experts from values in 64 bits, one at a time, by a whole wave: lane j's expert.
 // It is the definition of the choice, and what the 32-bit choice leaves to it where its values are too
-// close to tell the order, too far from the best, or no numbers.  value: E + G doubles of LDS, in which
-// the row's logits stand; m: their maximum; sum: of their exponentials, set here if `exps`.
-// Kept as loops: the code is cold, and fetching it unrolled took longer than running it.
-__device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool exps, int lane, float m, double &sum,
-                                        double *value) {
+// close to tell the order, too far from the best, or no numbers.  l[v], bias[v]: of expert 64 * v + lane
+// (-inf past the last); m: the logits' maximum; sum: of their exponentials, set here if `exps`; value:
+// E + G doubles of LDS (groups).  One row is 5 us of latency, which a launch sees once, at its end.
+template <int V>
+__device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool exps, int lane, const float (&l)[V],
+                                        const float (&bias)[V], float m, double &sum, double *value) {
     const int E = a.E, G = a.groups, S = E / G;
+    double c[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) c[v] = (double)l[v];
     sum = 1.0;
-    if (exps) {
-        sum = 0.0;
-#pragma unroll 1
-        for (int e = lane; e < E; e += 64) sum += value[e] == kDead ? 0.0 : exp(value[e] - (double)m);
-        sum = seg_reduce<64>(sum, Sum());
-    }
-#pragma unroll 1
-    for (int e = lane; e < E; e += 64) {
-        double x = value[e];
-        if (x == kDead) continue;
-        if (!by_logit) {
-            const double t = exp(a.score == 0 ? x - (double)m : -x);
-            x = a.score == 0 ? t / sum : 1.0 / (1.0 + t);
-            if (a.bias) x += (double)a.bias[e];
+    if (!by_logit || exps) {
+        // exponentials, two at a time
+        double t[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) t[v] = a.score == 0 ? c[v] - (double)m : -c[v];
+        if (V < 2) {
+            t[0] = exp(t[0]);
+        } else {
+#pragma unroll
+            for (int v = 0; v + 1 < V; v += 2) {
+                const double x = exp(t[v]), y = exp(t[v + 1]);
+                t[v] = x;
+                t[v + 1] = y;
+            }
+            if (V % 2) t[V - 1] = exp(t[V - 1]);
         }
-        value[e] = x >= kLast ? x : kLast;
+        if (exps) {
+            sum = 0.0;
+#pragma unroll
+            for (int v = 0; v < V; v++) sum += l[v] == -INFINITY ? 0.0 : t[v];
+            sum = seg_reduce<64>(sum, Sum());
+        }
+        if (!by_logit)
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                // t / sum, or 1 / (1 + t)
+                const double x = (a.score == 0 ? t[v] : 1.0) / (a.score == 0 ? sum : 1.0 + t[v]);
+                c[v] = a.bias ? x + (double)bias[v] : x;
+            }
     }
-    wave_lds_sync();
+#pragma unroll
+    for (int v = 0; v < V; v++) c[v] = l[v] == -INFINITY ? kDead : c[v] >= kLast ? c[v] : kLast;
     if (G > 1) {
         double *score = value + E;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (64 * v + lane < E) value[64 * v + lane] = c[v];
+        wave_lds_sync();
         double mine = kDead;
         if (lane < G) {
             double b2 = kDead;
-#pragma unroll 4
+#pragma unroll 8
             for (int s = 0; s < S; s++) {
                 const double x = value[lane * S + s];
                 b2 = x > mine ? mine : x > b2 ? x : b2;
@@ -348,25 +370,24 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool 
         }
         wave_lds_sync();
         int before = 0;         // a group is kept if fewer than top_groups come before it
-#pragma unroll 4
+#pragma unroll 8
         for (int o = 0; o < G; o++) {
             const double x = score[o];
             before += x > mine || (x == mine && o < lane);
         }
-        if (lane < G && before >= a.top_groups)
-#pragma unroll 1
-            for (int s = 0; s < S; s++) value[lane * S + s] = kDead;
+        const uint64_t kept = __ballot(lane < G && before < a.top_groups);
         wave_lds_sync();
+#pragma unroll
+        for (int v = 0; v < V; v++) c[v] = kept >> ((uint32_t)(64 * v + lane) / (uint32_t)S & 63) & 1 ? c[v] : kDead;
     }
     int my_e = -1;
     for (int j = 0; j < a.k; j++) {
         double best = kDead;
         int be = 1 << 20;
-#pragma unroll 4
-        for (int e = lane; e < E; e += 64) {
-            const double x = value[e];
-            be = x > best ? e : be;
-            best = x > best ? x : best;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            be = c[v] > best ? 64 * v + lane : be;
+            best = c[v] > best ? c[v] : best;
         }
         // the wave's maximum as ordered bits, high word first; of equal values the lowest expert
         uint64_t u;
@@ -383,10 +404,9 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool 
         }
         int won = __builtin_amdgcn_readlane(be, __builtin_ctzll(who));
         if (who & (who - 1)) won = (int)~wave_max(on ? ~(uint32_t)be : 0u);
-        const bool any = won < E;
-        if (lane == j) my_e = any ? won : -1;
-        if (any && lane == 0) value[won] = kDead;
-        wave_lds_sync();
+        if (lane == j) my_e = won < E ? won : -1;
+#pragma unroll
+        for (int v = 0; v < V; v++) c[v] = 64 * v + lane == won ? kDead : c[v];
     }
     return my_e;
 }
@@ -739,20 +759,25 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         for (int n = 0; n < n0; n++) left &= left - 1;
         const int i = __ffsll(left) - 1;
         const int64_t t = t0 + i;
+        constexpr int VX = (L * V + 63) / 64;
+        float l[VX], bx[VX], m = -INFINITY;
         bool nan = false;
-        float m = -INFINITY;
-#pragma unroll 4
-        for (int e = wl; e < E; e += 64) {
-            const float x = one_logit(a, t, e);
-            nan |= x != x;
-            m = fmaxf(m, x);
-            row64[e] = (double)x;
+#pragma unroll
+        for (int v = 0; v < VX; v++) {
+            const int e = 64 * v + wl;
+            l[v] = one_logit(a, t, e < E ? e : 0);
+            bx[v] = a.bias && e < E ? bias[(e % V / kVec * L + e / V) * kVec + e % V % kVec] : 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < VX; v++) {
+            if (64 * v + wl >= E) l[v] = -INFINITY;
+            nan |= l[v] != l[v];
+            m = fmaxf(m, l[v]);
         }
         nan = __any(nan);
         m = seg_max<64>(m);
-        wave_lds_sync();
         double sum;
-        const int my_e = choose64(a, by_logit, exps, wl, m, sum, row64);
+        const int my_e = choose64<VX>(a, by_logit, exps, wl, l, bx, m, sum, row64);
         finish_row<64>(a, t, i, true, wl, my_e, nan, m, (float)sum, mask);
     }
     __syncthreads();
@@ -1166,8 +1191,8 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
         // masks; the bases (one chunk); the groups' keys and, for groups of no power of two, the values of
         // every row at once; or a row's values and its groups' in 64 bits for every wave
         const size_t rows = kRouteThreads / decltype(L)::value, E = a.E, G = a.groups;
-        size_t room = std::max(4 * E, kRouteThreads / 64 * 8 * (E + G));
-        if (G > 1) room = std::max(room, rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
+        size_t room = 4 * E;
+        if (G > 1) room = std::max(std::max(room, kRouteThreads / 64 * 8 * (E + G)), rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
         const size_t lds = 8 * ((E + 1) / 2 * 2) + room;
         auto go = [&](auto KP) {
             const auto kern = k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value>;
