@@ -258,7 +258,8 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
  *   k best choice values win, in falling order; equal ones go to the lower index.  Choice values are
  *   compared as computed in 64 bits; without a bias (and with group_sum 1 or one group) as the
  *   logits themselves.
- *   weight = scale * s, over the sum of the chosen s if renorm (the bias is in no weight).
+ *   weight = scale * s, over the sum of the chosen s if renorm (the bias is in no weight); scale is
+ *   between 1e-18 and 1e18 in magnitude.
  *   A logit of -infinity masks the expert.  A row with fewer live experts than k has experts -1 and
  *   weights 0 at the end, a row with valid[t] == 0 in all slots (its logits are ignored).  A NaN
  *   counts as the lowest of all live choices, and the weights of its row are NaN.
@@ -282,7 +283,9 @@ int pss_route_grad(const void *logits, int64_t ld, int64_t tokens, int32_t exper
                    int32_t score, int32_t renorm, double scale, const int32_t *chosen, const float *weights,
                    const float *slopes, const float *dweights, void *dlogits, void *stream);
 
-/* Rows into expert order: xs[pos[t, j]] = x[t]; 0 where the slot has no expert. */
+/* Rows into expert order: xs[pos[t, j]] = x[t]; 0 where the slot has no expert.  (In this and the next
+ * two, experts and pos are what pss_route gave; a place outside [0, tokens * k) counts as a slot
+ * without an expert, and its row is not written.) */
 int pss_dispatch(const void *x, int64_t ldx, int64_t tokens, int32_t k, int64_t cols, int32_t dtype,
                  const int32_t *experts, const int32_t *pos, void *xs, void *stream);
 /* Rows back: out[t] = residual[t] + dropout(sum of weights[t, j] * y[pos[t, j]] over the slots with

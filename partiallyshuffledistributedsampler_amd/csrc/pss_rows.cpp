@@ -99,7 +99,8 @@ namespace cpu {
 void dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows, int64_t cols,
              int32_t dtype, const Drop &d, const RowGather *g) {
     for (int64_t r = 0; r < rows; r++) {
-        const int64_t id = d.row0 + (d.ids ? (d.per_row ? d.ids[r] : d.ids[0] + r) : r);
+        const int64_t id = (int64_t)((uint64_t)d.row0 + (d.ids ? (uint64_t)d.ids[d.per_row ? r : 0] : 0u) +
+                                     (d.per_row ? 0u : (uint64_t)r));
         int64_t from = r;
         if (g) {
             const int32_t f = g->fpos[r] < 0 ? -1 - g->fpos[r] : g->fpos[r];
@@ -164,12 +165,14 @@ static int route_args(RouteArgs *a, const void *logits, int64_t ld, int64_t toke
     if (tokens > 0 && !logits) return set_error(PSS_EINVAL, "route: NULL logits");
     if (ld < 0) return set_error(PSS_EINVAL, "the row stride must be >= 0");
     if (score != PSS_SOFTMAX && score != PSS_SIGMOID) return set_error(PSS_EINVAL, "route: score must be PSS_SOFTMAX or PSS_SIGMOID");
-    if (!(std::fabs(scale) <= 3.0e38) || scale == 0.0) return set_error(PSS_EINVAL, "route: scale must be a finite number other than 0");
+    if (!(std::fabs(scale) >= 1e-18 && std::fabs(scale) <= 1e18))
+        return set_error(PSS_EINVAL, "route: scale must be a number between 1e-18 and 1e18 in magnitude");
     *a = RouteArgs{};
     a->logits = logits;
     a->ld = ld;
     a->T = tokens;
     a->E = experts;
+    a->chunk = route_chunk(tokens, experts);
     a->k = k;
     a->dtype = dtype;
     a->score = score;
@@ -180,7 +183,7 @@ static int route_args(RouteArgs *a, const void *logits, int64_t ld, int64_t toke
 
 int64_t pss_route_workspace(int64_t tokens, int32_t experts) {
     if (tokens < 0 || experts < 1) return 0;
-    const int64_t n = route_chunks(tokens);
+    const int64_t n = route_chunks(tokens, experts);
     return n > 1 ? (n * 12 + 4) * experts : 0;
 }
 
@@ -214,7 +217,7 @@ int pss_route(const void *logits, int64_t ld, int64_t tokens, int32_t experts, i
     a.pos = pos;
     a.src = src;
     if (need > 0) {
-        const int64_t n = route_chunks(tokens) * experts;
+        const int64_t n = route_chunks(tokens, experts) * experts;
         a.mask = (uint64_t *)ws;
         a.before = (int32_t *)(a.mask + n);
         a.totals = a.before + n;

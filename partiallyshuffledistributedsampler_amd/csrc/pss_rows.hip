@@ -72,8 +72,8 @@ __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
 
 // ---- dropout -------------------------------------------------------------------------------------
 __device__ __forceinline__ int64_t drop_row(const Drop &d, int64_t i) {
-    if (!d.ids) return d.row0 + i;
-    return d.row0 + (d.per_row ? d.ids[i] : d.ids[0] + i);
+    const uint64_t id = !d.ids ? (uint64_t)i : d.per_row ? (uint64_t)d.ids[i] : (uint64_t)d.ids[0] + (uint64_t)i;
+    return (int64_t)((uint64_t)d.row0 + id);        // (modulo 2^64)
 }
 
 // The eight draws of a block of columns of the row with id r.
@@ -424,6 +424,26 @@ __device__ __forceinline__ float group_value(uint32_t key) {
     return __uint_as_float(u);
 }
 
+// The two best of the values of aligned runs of lanes: a lane stands for `unit` values, a run for `all`
+// (both powers of two), the lanes hold their own two best.
+template <int L> __device__ __forceinline__ void join_best(int unit, int all, float &b1, float &b2) {
+    auto join = [&](auto I) {
+        if ((unit << decltype(I)::value) < all) {
+            const float o1 = partner<decltype(I)::value>(b1), o2 = partner<decltype(I)::value>(b2);
+            b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+            b1 = fmaxf(b1, o1);
+        }
+    };
+    join(std::integral_constant<int, 0>());
+    join(std::integral_constant<int, 1>());
+    join(std::integral_constant<int, 2>());
+    join(std::integral_constant<int, 3>());
+    if constexpr (L == 64) {
+        join(std::integral_constant<int, 4>());
+        join(std::integral_constant<int, 5>());
+    }
+}
+
 constexpr int kRouteThreads = 512;
 
 // Exclusive scan of v[0, E) in LDS by all threads; returns the total.
@@ -441,7 +461,7 @@ __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tm
     return (int32_t)run;
 }
 
-// Places of the slots of one chunk of 64 rows: rows of an expert in the order of the rows (mask[e]: the
+// Places of the slots of one chunk of up to 64 rows: rows of an expert in the order of the rows (mask[e]: the
 // chunk's rows that have it, base[e]: where its rows of this chunk begin), slots without an expert from
 // unused0 on.  All threads, at most two slots each; `first` holds 64 words.
 static_assert(kRouteChunk * kRouteMaxK <= 2 * kRouteThreads, "slots of a chunk");
@@ -511,7 +531,7 @@ __device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i,
     }
 }
 
-// One workgroup routes a chunk of 64 rows, L lanes a row and V experts a lane.  The choice runs on
+// One workgroup routes a chunk of up to 64 rows, L lanes a row and V experts a lane.  The choice runs on
 // 32-bit keys that hold value and expert (unique, so that maxima need no ties): of 16-bit logits the
 // order-preserving bits themselves, else the value's distance from a floor below the row's best, in 24
 // bits (22 beyond 256 experts).  Sorting networks of the KP >= k largest keys run in registers and
@@ -522,6 +542,7 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     extern __shared__ __align__(16) uint64_t lds[];
     __shared__ uint32_t scan_tmp[kRouteThreads / 64], first[64];
     __shared__ unsigned long long odd_rows;
+    __shared__ int wild;        // a bias is no number: groups are then summed by choose64 alone
     constexpr int kIndex = L * V <= 256 ? 8 : 10;
     constexpr uint32_t kIndexMask = (1u << kIndex) - 1, kExactMask = 0x1FFFu;
     const int E = a.E, k = a.k, G = a.groups, S = E / G;
@@ -532,8 +553,8 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     const int Gp = (G + 3) & ~3;
     uint32_t *score = (uint32_t *)room + (size_t)seg * Gp;                 // [segments][Gp], the last ones 0
     float *value = (float *)room + (size_t)(kRouteThreads / L) * Gp + (size_t)seg * (L * V);  // [segments][L * V]
-    const int64_t t0 = (int64_t)blockIdx.x * kRouteChunk;
-    const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
+    const int64_t t0 = (int64_t)blockIdx.x * a.chunk;
+    const int nt = (int)(a.T - t0 < a.chunk ? a.T - t0 : a.chunk);
     const bool by_logit = !a.bias && (G == 1 || a.group_sum == 1);
     const bool exact = by_logit && a.dtype != 0;                           // keys that lose nothing
     const bool exps = a.score == 0 && !(by_logit && a.renorm);             // softmax statistics wanted
@@ -541,14 +562,17 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     for (int i = threadIdx.x; i < E; i += kRouteThreads) mask[i] = 0;
     if (G > 1)
         for (int i = threadIdx.x; i < kRouteThreads / L * Gp; i += kRouteThreads) ((uint32_t *)room)[i] = 0;
-    if (threadIdx.x == 0) odd_rows = 0;
+    if (threadIdx.x == 0) { odd_rows = 0; wild = 0; }
+    __syncthreads();
     // (in LDS, value v of lane x at v / 4 * 4 * L + 4 * x + v % 4: registers are what limits the waves)
     __shared__ float bias[L * V < 64 ? 64 : L * V];
     constexpr int kVec = V < 4 ? V : 4;
     if (a.bias)
         for (int e = threadIdx.x; e < L * V; e += kRouteThreads) {
             const int x = e / V, v = e % V;
-            bias[(v / kVec * L + x) * kVec + v % kVec] = e < E ? a.bias[e] : 0.f;
+            const float b = e < E ? a.bias[e] : 0.f;
+            bias[(v / kVec * L + x) * kVec + v % kVec] = b;
+            if (G > 1 && !(fabsf(b) < 1e30f)) wild = 1;
         }
     auto add_bias = [&](float (&c)[V]) {
 #pragma unroll
@@ -598,6 +622,7 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
             if (a.bias) add_bias(c);
         }
         if (G > 1) {
+            odd |= wild != 0;
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = fmaxf(c[v], -INFINITY);      // (a median takes no NaN)
             // the two best of every group: a lane's values one by one, then across lanes, or through LDS
@@ -616,34 +641,29 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
                         b1 = b2 = -INFINITY;
                     }
                 }
-                auto join = [&](auto I) {
-                    if ((V << decltype(I)::value) < S) {
-                        const float o1 = partner<decltype(I)::value>(b1), o2 = partner<decltype(I)::value>(b2);
-                        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
-                        b1 = fmaxf(b1, o1);
-                    }
-                };
-                join(std::integral_constant<int, 0>());
-                join(std::integral_constant<int, 1>());
-                join(std::integral_constant<int, 2>());
-                join(std::integral_constant<int, 3>());
-                if constexpr (L == 64) {
-                    join(std::integral_constant<int, 4>());
-                    join(std::integral_constant<int, 5>());
-                }
+                join_best<L>(V, S, b1, b2);
                 if (S > V && ((lane * V) & (S - 1)) == 0 && lane * V < E) flush(lane * V);
             } else {
 #pragma unroll
                 for (int v = 0; v < V; v++) value[lane * V + v] = c[v];
                 wave_lds_sync();
-                for (int g = lane; g < G; g += L) {
+                // `share` lanes a group
+                int share = 1;
+                while (2 * share * G <= L) share *= 2;
+                for (int g0 = 0; g0 < G; g0 += L / share) {
+                    const int g = g0 + lane / share;
                     float b1 = -INFINITY, b2 = -INFINITY;
-                    for (int s = 0; s < S; s++) {
-                        const float x = value[g * S + s];
-                        b2 = __builtin_amdgcn_fmed3f(b1, b2, x);
-                        b1 = fmaxf(b1, x);
+                    if (g < G) {
+#pragma unroll 4
+                        for (int s = lane & (share - 1); s < S; s += share) {
+                            const float x = value[g * S + s];
+                            b2 = __builtin_amdgcn_fmed3f(b1, b2, x);
+                            b1 = fmaxf(b1, x);
+                        }
                     }
-                    score[g] = group_key(a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1, g);
+                    join_best<L>(1, share, b1, b2);
+                    if (g < G && !(lane & (share - 1)))
+                        score[g] = group_key(a.group_sum == 2 && b2 > -INFINITY ? b1 + b2 : b1, g);
                 }
             }
             wave_lds_sync();
@@ -839,8 +859,8 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
     const int E = a.E;
     uint64_t *mask = lds;                       // [E]
     int32_t *base = (int32_t *)(mask + E);      // [E]
-    const int64_t c = blockIdx.x, t0 = c * kRouteChunk;
-    const int nt = (int)(a.T - t0 < kRouteChunk ? a.T - t0 : kRouteChunk);
+    const int64_t c = blockIdx.x, t0 = c * a.chunk;
+    const int nt = (int)(a.T - t0 < a.chunk ? a.T - t0 : a.chunk);
     // exclusive sums over the experts: all their rows, and (high half) this chunk's predecessors' rows
     uint64_t run = 0;
     for (int e0 = 0; e0 < E; e0 += kRouteThreads) {
@@ -937,7 +957,8 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const
 
 // ---- rows moved: gather, dispatch, combine -------------------------------------------------------
 // L lanes of a 256-thread workgroup share one row (16, 64 or all 256), eight columns a lane and step;
-// gridDim.y workgroups share its columns where there are few rows.
+// gridDim.y workgroups share its columns where there are few rows.  A place outside the T * k rows (a
+// plan that route did not make) is taken as a slot without an expert, and nothing is written there.
 template <int L>
 __device__ __forceinline__ int64_t first_row() {
     const int sub = L >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : (int)threadIdx.x / L;
@@ -965,6 +986,7 @@ __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data,
 
 template <typename T, int L>
 __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restrict__ x, int64_t ldx, T *__restrict__ xs) {
+    const uint32_t places = (uint32_t)(m.T * m.k);
     for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
         const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
         for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
@@ -972,6 +994,7 @@ __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restric
             const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             load(x + t * ldx + c, m.D - c, v);
             for (int j = 0; j < m.k; j++) {
+                if ((uint32_t)pos[j] >= places) continue;
                 T *to = xs + (int64_t)pos[j] * m.D + c;
                 if (e[j] >= 0) store(to, m.D - c, v);
                 else store(to, m.D - c, zero);
@@ -985,6 +1008,7 @@ __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restric
 template <typename T, int L, int KU, bool NT>
 __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict__ y, const float *__restrict__ w,
                                                  const T *__restrict__ res, int64_t ldr, Drop d, T *__restrict__ out) {
+    const uint32_t places = (uint32_t)(m.T * m.k);
     for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
         const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
         const int64_t id = d.drop ? drop_row(d, t) : 0;
@@ -997,13 +1021,14 @@ __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict
 #pragma unroll
                 for (int u = 0; u < KU; u++) {
                     const int j = j0 + u < m.k ? j0 + u : j0;
-                    load<NT>(y + (int64_t)pos[j] * m.D + c, m.D - c, v[u]);
+                    const uint32_t at = (uint32_t)pos[j] < places ? (uint32_t)pos[j] : 0u;
+                    load<NT>(y + (int64_t)at * m.D + c, m.D - c, v[u]);
                 }
                 if (d.drop && j0 == 0) dr = draw8(d, id, (uint32_t)(c >> 3));   // while the rows come
 #pragma unroll
                 for (int u = 0; u < KU; u++) {
                     const int j = j0 + u < m.k ? j0 + u : j0;
-                    const bool on = j0 + u < m.k && e[j] >= 0;
+                    const bool on = j0 + u < m.k && e[j] >= 0 && (uint32_t)pos[j] < places;
                     const float wj = w ? w[t * m.k + j] : 1.f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) acc[i] = on ? fmaf(wj, v[u][i], acc[i]) : acc[i];
@@ -1028,17 +1053,20 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
                                                       const T *__restrict__ y, const float *__restrict__ w, Drop d,
                                                       T *__restrict__ dy, float *__restrict__ dw) {
     constexpr int KU = KM < 8 ? KM : 8;
+    const uint32_t rows = (uint32_t)(m.T * m.k);
     __shared__ float part[L > 64 ? 4 : 1][KM];
     for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
         const int64_t id = d.drop ? drop_row(d, t) : 0;
         float dot[KM], wt[KM];
         int32_t pos[KM];
-        bool on[KM];
+        bool on[KM], in[KM];
 #pragma unroll
         for (int j = 0; j < KM; j++) {
             const int64_t slot = t * m.k + (j < m.k ? j : 0);
-            on[j] = experts[slot] >= 0;
-            pos[j] = places[slot];
+            const uint32_t at = (uint32_t)places[slot];
+            on[j] = experts[slot] >= 0 && at < rows;
+            in[j] = at < rows;
+            pos[j] = at < rows ? (int32_t)at : 0;
             wt[j] = w[slot];
             dot[j] = 0.f;
         }
@@ -1062,6 +1090,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
 #pragma unroll
                     for (int u = 0; u < KU; u++) {
                         if (j0 + u >= m.k) break;
+                        if (!in[j0 + u]) continue;
                         float o[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++) o[i] = on[j0 + u] ? wt[j0 + u] * g[i] : 0.f;
@@ -1080,7 +1109,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
                 for (int j = 0; j < KM; j++) part[threadIdx.x >> 6][j] = dot[j];
             __syncthreads();
             const int j = threadIdx.x;
-            if (j < m.k) dw[t * m.k + j] = experts[t * m.k + j] >= 0 ? (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]) : 0.f;
+            if (j < m.k) dw[t * m.k + j] = experts[t * m.k + j] >= 0 && (uint32_t)places[t * m.k + j] < rows ? (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]) : 0.f;
         } else {
 #pragma unroll
             for (int j = 0; j < KM; j++)
@@ -1184,7 +1213,7 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
 }
 
 hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
-    const int64_t chunks = route_chunks(a.T);
+    const int64_t chunks = route_chunks(a.T, a.E);
     const int S = a.E / a.groups;
     hipError_t err = hipSuccess;
     by_width(a.E, [&](auto L, auto V) {

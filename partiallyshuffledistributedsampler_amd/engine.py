@@ -188,6 +188,9 @@ class IndexEngine:
                 raise ValueError("gather: out must be contiguous, of the data's dtype, on the engine's device")
             if not 0.0 <= p <= 1.0:
                 raise ValueError("p must be in [0, 1], got %r" % p)
+            if off.numel() != n or base_rows.numel() < self.num_files:
+                raise ValueError("gather: file_pos and offset must be of one length, base_rows must have an "
+                                 "entry for each of the %d files" % self.num_files)
             row0, ids = _row_ids(rows)
             if ids is not None:
                 if ids.dtype != torch.int64 or ids.device != d or ids.numel() not in (1, n):

@@ -103,7 +103,7 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     groups       consecutive experts form this many equal groups, and only the top_groups groups of
                  the highest value -- the sum of their group_sum (1 or 2) best -- take part
     renormalise  a row's weights are divided by the sum of its chosen scores
-    scale        factor of all weights
+    scale        factor of all weights (1e-18 to 1e18 in magnitude)
     valid        [T] bool: rows that are padding get no expert
 
     The best choice first, ties to the lower index.  A logit of -inf masks the expert; a row with

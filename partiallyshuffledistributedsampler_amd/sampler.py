@@ -383,8 +383,8 @@ class _PartialShuffleSampler(Sampler):
         """The dropout key (ops.dropout, ops.combine) of this sampler's seed, current epoch and
         logical rank at one place (`site`) of a model: with a sample's position in the rank's
         stream as its row's id, a run resumed from state_dict() drops what the uninterrupted one
-        would have dropped, for any batch size and number of GPUs.  device_batches(p=...) uses
-        site 0."""
+        would have dropped, for any batch size and number of GPUs (and the same seed, in the exact
+        order too).  device_batches(p=...) uses site 0."""
         from .ops import dropout_key
         if not self._iterated:
             raise RuntimeError("call iter(sampler) first")

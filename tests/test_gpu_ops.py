@@ -108,6 +108,10 @@ def test_gather_with_dropout(dtype, shape):
         eng.gather(data, base, fpos, off, out=out[:7], p=0.3)
     with pytest.raises(TypeError, match="float32"):
         eng.gather(data.to(torch.float64), base, fpos, off, p=0.3)
+    with pytest.raises(ValueError, match="one length"):
+        eng.gather(data, base, fpos, off[:, :5], p=0.3)
+    with pytest.raises(ValueError, match="one length"):
+        eng.gather(data, base[:4], fpos, off, p=0.3)
     eng.close()
 
 
@@ -165,6 +169,9 @@ SHAPES = [
     (130, 40, 10, dict(groups=40, top_groups=20, group_sum=2, bias=True)),
     (64, 512, 8, dict(groups=64, top_groups=3, group_sum=1, bias=True, score="sigmoid")),
     (70, 320, 12, dict(groups=2, top_groups=1, group_sum=2, bias=True, score="softmax")),
+    (150, 394, 1, dict(groups=2, top_groups=1, group_sum=2, bias=True, score="sigmoid", renormalise=False)),
+    (150, 36, 3, dict(groups=4, top_groups=3, group_sum=2)), (70, 300, 4, dict(groups=60, top_groups=10, group_sum=2)),
+    (70, 264, 4, dict(groups=24, top_groups=10, bias=True)), (70, 90, 4, dict(groups=30, top_groups=4, group_sum=2)),
     (40, 257, 16, dict(bias=True)), (33, 600, 7, dict(score="sigmoid", bias=True, renormalise=False)),
     (20, 1024, 16, dict(groups=32, top_groups=32, group_sum=2, score="sigmoid")), (3, 1024, 1, dict(renormalise=False)),
 ]
@@ -276,6 +283,42 @@ def test_route_of_nan_rows_stays_in_range(score, bias, groups):
     if not bias and groups == 1:
         assert 4 not in e[1].tolist() and e[2].tolist() == [0, 1, 2, 3] and e[3, 0] == 7
     assert torch.equal(torch.sort(r.pos.reshape(-1))[0], torch.arange(48, dtype=torch.int32, device=dev()))
+
+
+def test_route_of_padding_alone_and_of_a_zero_router():
+    for T, E, kw in ((300, 40, {}), (9, 7, dict(bias=torch.zeros(7, device=dev()))), (200, 300, dict(groups=4, top_groups=2))):
+        l = rnd(T, T, E)
+        r = check_route(l, 3, valid=torch.zeros(T, dtype=torch.bool, device=dev()), **kw)
+        assert (r.experts == -1).all() and (r.offsets == 0).all() and (r.weights == 0).all()
+        check_route(torch.zeros(T, E, device=dev()), 3, **kw)
+
+
+@pytest.mark.parametrize("bias", [1e9, -1e9, 1e5, 100.0])
+@pytest.mark.parametrize("groups", [1, 5])
+def test_route_large_biases(bias, groups):
+    # experts switched off or forced by their bias
+    b = rnd(1, 60, scale=0.1)
+    b[::7] += bias
+    check_route(rnd(2, 300, 60), 5, bias=b, score="sigmoid", groups=groups, top_groups=max(1, groups // 2), group_sum=2)
+    check_route(rnd(3, 300, 60, dtype="bf16"), 5, bias=b, groups=groups, top_groups=max(1, groups // 2))
+
+
+def test_plan_that_route_did_not_make_writes_nowhere_else():
+    T, k, D = 6, 2, 40
+    r = ops.route(rnd(1, T, 4), k)
+    x, y = rnd(2, T, D), rnd(3, T * k, D).requires_grad_()
+    pos = r.pos.clone()
+    pos[2, 1], pos[4, 0] = -5, 1 << 30
+    bad = r._replace(pos=pos, weights=r.weights.detach().requires_grad_())
+    good = r._replace(experts=r.experts.clone(), weights=r.weights.detach())
+    good.experts[2, 1] = good.experts[4, 0] = -1
+    xs, want = ops.dispatch(x, bad), ops.dispatch(x, good)
+    on = [p for i, p in enumerate(r.pos.reshape(-1).tolist()) if i not in (5, 8)]
+    assert torch.equal(xs[on], want[on])
+    out = ops.combine(y, bad)
+    assert torch.equal(out, ops.combine(y, good))
+    dy, dw = torch.autograd.grad(out, (y, bad.weights), torch.ones(T, D, device=dev()))
+    assert dw[2, 1] == 0 and dw[4, 0] == 0
 
 
 def test_route_strided_logits_and_no_gradient():
@@ -539,7 +582,7 @@ def test_gpu_refusals():
         with pytest.raises(ValueError, match="valid"):
             ops.route(l, 2, valid=valid)
     for kw in (dict(k=0), dict(k=9), dict(k=2, groups=3), dict(k=2, groups=4, top_groups=5), dict(k=3, groups=4),
-               dict(k=2, group_sum=0), dict(k=2, scale=0.0), dict(k=2, scale=float("inf"))):
+               dict(k=2, group_sum=0), dict(k=2, scale=0.0), dict(k=2, scale=float("inf")), dict(k=2, scale=1e-30)):
         with pytest.raises(RuntimeError, match="route"):
             ops.route(l, **kw)
     with pytest.raises(TypeError, match="Routing"):
