@@ -1047,7 +1047,7 @@ __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict
 
 // One pass over g = dropout(dout): KU products with rows of y and KU rows of dy at a time.  The lanes
 // of a row hold partial products of all its slots; they are joined after the last column.
-template <typename T, int L, int KM>
+template <typename T, int L, int KM, bool NT>
 __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t *__restrict__ experts,
                                                       const int32_t *__restrict__ places, const T *__restrict__ dout, int64_t ldo,
                                                       const T *__restrict__ y, const float *__restrict__ w, Drop d,
@@ -1080,7 +1080,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
                 if (dw) {
                     float v[KU][8];
 #pragma unroll
-                    for (int u = 0; u < KU; u++) load(y + (int64_t)pos[j0 + u] * m.D + c, m.D - c, v[u]);
+                    for (int u = 0; u < KU; u++) load<NT>(y + (int64_t)pos[j0 + u] * m.D + c, m.D - c, v[u]);
 #pragma unroll
                     for (int u = 0; u < KU; u++)
 #pragma unroll
@@ -1146,8 +1146,9 @@ void by_width(int E, F f) {
 // Whether a pass over so many bytes goes past the caches: beyond the 256 MB of the Infinity Cache
 // nothing of it can be found there later.  Measured past / through: dropout 16384 x 8192 bf16 with
 // residual 131 / 157 us, without 91 / 94; gather of 65536 x 2048 bf16 99 / 125; combine of
-// 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16 (17 MB) 7.8 / 7.4.  Dispatch and
-// the combine's gradient write eight rows for one read and are slower past them (249 / 223, 474 / 458).
+// 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16 (17 MB) 7.8 / 7.4; the reads of y of
+// the combine's gradient (16384 x 8 x 4096) 480 / 495.  Rows written for one read are slower past them
+// (dispatch 249 / 223, the gradient's writes 525 / 495).
 static bool past_caches(int64_t bytes) { return bytes > ((int64_t)256 << 20); }
 
 template <typename F>
@@ -1293,8 +1294,11 @@ hipError_t launch_combine_grad(const MoveArgs &m, const void *dout, int64_t ldo,
         by_row(m.T, m.D, [&](auto L, dim3 grid) {
             grid.y = 1;     // the products run over all columns
             by_slots(m.k, [&](auto KM) {
-                hipLaunchKernelGGL((k_combine_grad<T, decltype(L)::value, decltype(KM)::value>), grid, dim3(256), 0, s,
-                                   m, m.experts, m.pos, (const T *)dout, ldo, (const T *)y, w, d, (T *)dy, dw);
+                by_flag(past_caches(m.T * (2 * m.k + 1) * m.D * (int64_t)sizeof(T)), [&](auto NT) {
+                    hipLaunchKernelGGL((k_combine_grad<T, decltype(L)::value, decltype(KM)::value, decltype(NT)::value>),
+                                       grid, dim3(256), 0, s, m, m.experts, m.pos, (const T *)dout, ldo, (const T *)y,
+                                       w, d, (T *)dy, dw);
+                });
             });
         });
     });
