@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
 }
 
 // ---- routing -------------------------------------------------------------------------------------
-// The lanes of a segment (16 or 64 of a wave) share one row; reductions stay inside the segment.  Step
+// The lanes of a segment (4, 8, 16 or 64 of a wave) share one row; reductions stay inside the segment.  Step
 // i joins lanes that hold the same after the steps before: 1 and 2 apart, then the halves of 8 and 16
 // mirrored (DPP, no LDS), then 16 and 32 apart.
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_mov(uint32_t x) {
@@ -159,8 +159,8 @@ template <int L, typename T, typename F>
 __device__ __forceinline__ T seg_reduce(T v, F f) {
     v = f(v, partner<0>(v));
     v = f(v, partner<1>(v));
-    v = f(v, partner<2>(v));
-    v = f(v, partner<3>(v));
+    if constexpr (L >= 8) v = f(v, partner<2>(v));
+    if constexpr (L >= 16) v = f(v, partner<3>(v));
     if constexpr (L == 64) {
         v = f(v, partner<4>(v));
         v = f(v, partner<5>(v));
@@ -286,8 +286,10 @@ __device__ __forceinline__ void seg_top(const uint32_t *key, uint32_t first, uin
     };
     step(std::integral_constant<int, 0>());
     step(std::integral_constant<int, 1>());
-    step(std::integral_constant<int, 2>());
-    step(std::integral_constant<int, 3>());
+    if constexpr (L >= 16) {
+        step(std::integral_constant<int, 2>());
+        step(std::integral_constant<int, 3>());
+    }
     if constexpr (L == 64) {
         step(std::integral_constant<int, 4>());
         step(std::integral_constant<int, 5>());
@@ -436,24 +438,26 @@ template <int L> __device__ __forceinline__ void join_best(int unit, int all, fl
     };
     join(std::integral_constant<int, 0>());
     join(std::integral_constant<int, 1>());
-    join(std::integral_constant<int, 2>());
-    join(std::integral_constant<int, 3>());
+    if constexpr (L >= 16) {
+        join(std::integral_constant<int, 2>());
+        join(std::integral_constant<int, 3>());
+    }
     if constexpr (L == 64) {
         join(std::integral_constant<int, 4>());
         join(std::integral_constant<int, 5>());
     }
 }
 
-constexpr int kRouteThreads = 512;
+constexpr int kPlaceThreads = 512;
 
-// Exclusive scan of v[0, E) in LDS by all threads; returns the total.
-__device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tmp) {
+// Exclusive scan of v[0, E) in LDS by all NT threads; returns the total.
+template <int NT> __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tmp) {
     uint32_t run = 0;
-    for (int e0 = 0; e0 < E; e0 += kRouteThreads) {
+    for (int e0 = 0; e0 < E; e0 += NT) {
         const int e = e0 + threadIdx.x;
         uint32_t total;
         const uint32_t x = e < E ? (uint32_t)v[e] : 0u;
-        const uint32_t pre = block_excl_scan<kRouteThreads>(x, scan_tmp, total);
+        const uint32_t pre = block_excl_scan<NT>(x, scan_tmp, total);
         if (e < E) v[e] = (int32_t)(run + pre);
         run += total;
     }
@@ -463,16 +467,17 @@ __device__ __forceinline__ int32_t scan_lds(int32_t *v, int E, uint32_t *scan_tm
 
 // Places of the slots of one chunk of up to 64 rows: rows of an expert in the order of the rows (mask[e]: the
 // chunk's rows that have it, base[e]: where its rows of this chunk begin), slots without an expert from
-// unused0 on.  All threads, at most two slots each; `first` holds 64 words.
-static_assert(kRouteChunk * kRouteMaxK <= 2 * kRouteThreads, "slots of a chunk");
+// unused0 on.  All NT threads, at most kRouteChunk * kRouteMaxK / NT slots each; `first` holds 64 words.
+template <int NT>
 __device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int nt, const uint64_t *mask,
                                             const int32_t *base, int32_t unused0, uint32_t *first) {
+    constexpr int kPer = kRouteChunk * kRouteMaxK / NT;
     const int k = a.k, n = nt * k;
-    int e[2];
+    int e[kPer];
     bool none = false;
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const int i = threadIdx.x + q * kRouteThreads;
+    for (int q = 0; q < kPer; q++) {
+        const int i = threadIdx.x + q * NT;
         e[q] = i < n ? a.experts[t0 * k + i] : 0;
         none |= e[q] < 0;
     }
@@ -488,8 +493,8 @@ __device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int 
         __syncthreads();
     }
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const int i = threadIdx.x + q * kRouteThreads;
+    for (int q = 0; q < kPer; q++) {
+        const int i = threadIdx.x + q * NT;
         if (i >= n) break;
         const int t = i / k, j = i - t * k;
         const int64_t slot = t0 * k + i;
@@ -500,34 +505,34 @@ __device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int 
     }
 }
 
-// Weights and outputs of a row (bit i of its chunk) with lane j's expert my_e, of which lanes < k hold
-// one; m, sum: the softmax statistics (scores not renormalised).  Softmax is exp(l - max) / sum,
-// renormalised over the chosen alone; the ratio of the chosen sigmoids comes from their logarithms,
-// which neither under- nor overflow.
-template <int L>
-__device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i, bool write, int lane, int my_e, bool nan,
-                                           float m, float sum, uint64_t *mask) {
+// Weight of the slot of a thread, KP threads a row: e its expert (0xFFFF: none); m, sum: the row's softmax
+// statistics (scores not renormalised).  Softmax is exp(l - max) / sum, renormalised over the chosen
+// alone; the ratio of the chosen sigmoids comes from their logarithms, which neither under- nor overflow.
+template <int KP>
+__device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i, int j, int e, bool nan, float m,
+                                            float sum, uint64_t *mask) {
+    const bool used = j < a.k && e != 0xFFFF;
+    const float lw = used ? one_logit(a, t, e) : -INFINITY;
     float w = 0.f;
-    const bool used = my_e >= 0 && lane < a.k;
-    const float lw = used ? one_logit(a, t, my_e) : -INFINITY;
     if (a.renorm) {
         // (the logarithm is off by 2^-24 absolutely: its argument is in [1, 2])
         const float z = !used ? -INFINITY : a.score == 0 ? lw
                         : fminf(lw, 0.f) - 0.69314718f * __builtin_amdgcn_logf(1.f + fast_exp(-fabsf(lw)));
-        const float zm = seg_max<L>(z);
+        const float zm = seg_max<KP>(z);
         w = used ? fast_exp(z - zm) : 0.f;
-        const float ws = seg_reduce<L>(w, Sum());
+        const float ws = seg_reduce<KP>(w, Sum());
         w = used ? w / ws * a.scale : 0.f;
     } else if (used) {
         w = a.scale * (a.score == 0 ? fast_exp(lw - m) / sum : 1.f / (1.f + fast_exp(-lw)));
     }
     if (used && nan) w = NAN;
-    if (write && lane < a.k) {
-        a.experts[t * a.k + lane] = my_e;
-        a.weights[t * a.k + lane] = w;
+    if (j < a.k) {
+        const int64_t slot = t * a.k + j;
+        a.experts[slot] = used ? e : -1;
+        a.weights[slot] = w;
         // 1 - sigmoid, for the gradient: its rows would else be read again for k values each
-        if (a.slopes) a.slopes[t * a.k + lane] = used ? 1.f / (1.f + fast_exp(lw)) : 0.f;
-        if (my_e >= 0) atomicOr((unsigned long long *)&mask[my_e], 1ull << i);
+        if (a.slopes) a.slopes[slot] = used ? 1.f / (1.f + fast_exp(lw)) : 0.f;
+        if (used) atomicOr((unsigned long long *)&mask[e], 1ull << i);
     }
 }
 
@@ -536,12 +541,15 @@ __device__ __forceinline__ void finish_row(const RouteArgs &a, int64_t t, int i,
 // order-preserving bits themselves, else the value's distance from a floor below the row's best, in 24
 // bits (22 beyond 256 experts).  Sorting networks of the KP >= k largest keys run in registers and
 // across lanes.  A row where two neighbours of the result, or the last chosen and the first not, are
-// nearer than the keys' and the scores' error is left to choose64 after the others.
-template <int L, int V, int KP>
-__global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
+// nearer than the keys' and the scores' error is left to choose64 after the others.  Weights come last,
+// KP threads a row.
+template <int L, int V, int KP, int kThreads>
+__global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
     extern __shared__ __align__(16) uint64_t lds[];
-    __shared__ uint32_t scan_tmp[kRouteThreads / 64], first[64];
-    __shared__ unsigned long long odd_rows;
+    __shared__ uint32_t scan_tmp[kThreads / 64], first[64];
+    __shared__ unsigned long long odd_rows, nan_rows;
+    __shared__ __align__(16) uint16_t chosen[kRouteChunk * KP];
+    __shared__ float2 stat[kRouteChunk];
     __shared__ int wild;        // a bias is no number: groups are then summed by choose64 alone
     constexpr int kIndex = L * V <= 256 ? 8 : 10;
     constexpr uint32_t kIndexMask = (1u << kIndex) - 1, kExactMask = 0x1FFFu;
@@ -552,23 +560,23 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
     double *room = (double *)(mask + (E + 1) / 2 * 2);                     // 16-byte aligned; groups alone:
     const int Gp = (G + 3) & ~3;
     uint32_t *score = (uint32_t *)room + (size_t)seg * Gp;                 // [segments][Gp], the last ones 0
-    float *value = (float *)room + (size_t)(kRouteThreads / L) * Gp + (size_t)seg * (L * V);  // [segments][L * V]
+    float *value = (float *)room + (size_t)(kThreads / L) * Gp + (size_t)seg * (L * V);  // [segments][L * V]
     const int64_t t0 = (int64_t)blockIdx.x * a.chunk;
     const int nt = (int)(a.T - t0 < a.chunk ? a.T - t0 : a.chunk);
     const bool by_logit = !a.bias && (G == 1 || a.group_sum == 1);
     const bool exact = by_logit && a.dtype != 0;                           // keys that lose nothing
     const bool exps = a.score == 0 && !(by_logit && a.renorm);             // softmax statistics wanted
     const uint32_t inv = ((1u << 20) + S - 1) / S;                         // e / S = e * inv >> 20, e < 1024
-    for (int i = threadIdx.x; i < E; i += kRouteThreads) mask[i] = 0;
+    for (int i = threadIdx.x; i < E; i += kThreads) mask[i] = 0;
     if (G > 1)
-        for (int i = threadIdx.x; i < kRouteThreads / L * Gp; i += kRouteThreads) ((uint32_t *)room)[i] = 0;
-    if (threadIdx.x == 0) { odd_rows = 0; wild = 0; }
+        for (int i = threadIdx.x; i < kThreads / L * Gp; i += kThreads) ((uint32_t *)room)[i] = 0;
+    if (threadIdx.x == 0) { odd_rows = nan_rows = 0; wild = 0; }
     __syncthreads();
     // (in LDS, value v of lane x at v / 4 * 4 * L + 4 * x + v % 4: registers are what limits the waves)
     __shared__ float bias[L * V < 64 ? 64 : L * V];
     constexpr int kVec = V < 4 ? V : 4;
     if (a.bias)
-        for (int e = threadIdx.x; e < L * V; e += kRouteThreads) {
+        for (int e = threadIdx.x; e < L * V; e += kThreads) {
             const int x = e / V, v = e % V;
             const float b = e < E ? a.bias[e] : 0.f;
             bias[(v / kVec * L + x) * kVec + v % kVec] = b;
@@ -579,7 +587,7 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         for (int v = 0; v < V; v++) c[v] += bias[(v / kVec * L + lane) * kVec + v % kVec];
     };
     __syncthreads();
-    for (int i0 = 0; i0 < nt; i0 += kRouteThreads / L) {
+    for (int i0 = 0; i0 < nt; i0 += kThreads / L) {
         asm volatile("" : "+v"(lane));      // what depends on the lane is made anew for every row, not kept
         const int i = i0 + seg;
         const bool row = i < nt;
@@ -735,14 +743,7 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         }
         uint32_t top[KP];
         seg_top<L, V, KP>(key, lane * V, top);
-        uint32_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < KP; j++) mine = lane == j ? top[j] : mine;
-        int my_e;
-        if (exact) {
-            my_e = mine ? (int)(kExactMask - (mine & kExactMask)) : -1;
-        } else {
-            my_e = (int)(kIndexMask - (mine & kIndexMask));
+        if (!exact) {
             // neighbours nearer than eps, or one at the floor; then the best key that was not chosen
             uint32_t last = 0;
 #pragma unroll
@@ -765,16 +766,27 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
             odd |= (float)((last >> kIndex) - (rest >> kIndex)) < eps;
         }
         odd = seg_reduce<L>((int)odd, Or()) != 0 && on;
-        if (!on || odd || lane >= k) my_e = -1;     // (a key at the floor may be of no expert at all)
-        if (odd && lane == 0) atomicOr(&odd_rows, 1ull << i);
-        finish_row<L>(a, t, i, row && !odd, lane, my_e, false, m, sum, mask);
+        if (row && lane == 0) {
+            // (a key at the floor may be of no expert at all: choose64 writes the odd rows' experts)
+            const uint32_t field = exact ? kExactMask : kIndexMask;
+            uint32_t pair[KP / 2];
+#pragma unroll
+            for (int j = 0; j < KP; j += 2) {
+                const uint32_t e = on && top[j] ? field - (top[j] & field) : 0xFFFFu;
+                const uint32_t f = on && top[j + 1] ? field - (top[j + 1] & field) : 0xFFFFu;
+                pair[j / 2] = e | f << 16;
+            }
+            __builtin_memcpy(__builtin_assume_aligned(chosen + i * KP, KP >= 8 ? 16 : 8), pair, sizeof(pair));
+            if (exps) stat[i] = make_float2(m, sum);
+            if (odd) atomicOr(&odd_rows, 1ull << i);
+        }
     }
     __syncthreads();
     // the rows left, a wave each
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
     const int odds = __popcll(odd_rows);
     double *row64 = room + (size_t)wave * (E + G);
-    for (int n0 = wave; n0 < odds; n0 += kRouteThreads / 64) {
+    for (int n0 = wave; n0 < odds; n0 += kThreads / 64) {
         unsigned long long left = odd_rows;
         for (int n = 0; n < n0; n++) left &= left - 1;
         const int i = __ffsll(left) - 1;
@@ -798,21 +810,31 @@ __global__ __launch_bounds__(kRouteThreads, 4) void k_route(RouteArgs a) {
         m = seg_max<64>(m);
         double sum;
         const int my_e = choose64<VX>(a, by_logit, exps, wl, l, bx, m, sum, row64);
-        finish_row<64>(a, t, i, true, wl, my_e, nan, m, (float)sum, mask);
+        if (wl < KP) chosen[i * KP + wl] = (uint16_t)(wl < k && my_e >= 0 ? my_e : 0xFFFF);
+        if (wl == 0) {
+            if (exps) stat[i] = make_float2(m, (float)sum);
+            if (nan) atomicOr(&nan_rows, 1ull << i);
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < nt * KP; x += kThreads) {
+        const int i = x / KP, j = x % KP;
+        const float2 ms = exps ? stat[i] : make_float2(0.f, 1.f);
+        finish_slot<KP>(a, t0 + i, i, j, chosen[x], nan_rows >> i & 1, ms.x, ms.y, mask);
     }
     __syncthreads();
     if (a.mask) {
-        for (int e = threadIdx.x; e < E; e += kRouteThreads) a.mask[(int64_t)blockIdx.x * E + e] = mask[e];
+        for (int e = threadIdx.x; e < E; e += kThreads) a.mask[(int64_t)blockIdx.x * E + e] = mask[e];
         return;
     }
     // the only chunk: places at once
     int32_t *base = (int32_t *)(mask + E);
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) base[e] = __popcll(mask[e]);
+    for (int e = threadIdx.x; e < E; e += kThreads) base[e] = __popcll(mask[e]);
     __syncthreads();
-    const int32_t total = scan_lds(base, E, scan_tmp);
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) a.offsets[e] = base[e];
+    const int32_t total = scan_lds<kThreads>(base, E, scan_tmp);
+    for (int e = threadIdx.x; e < E; e += kThreads) a.offsets[e] = base[e];
     if (threadIdx.x == 0) a.offsets[E] = total;
-    place_chunk(a, t0, nt, mask, base, total, first);
+    place_chunk<kThreads>(a, t0, nt, mask, base, total, first);
 }
 
 // Rows of every expert in the chunks before each chunk, and in all chunks: a workgroup takes 8 experts,
@@ -851,10 +873,10 @@ __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict_
 }
 
 // Places of one chunk's slots.  Without the sums of k_route_scan a workgroup counts all chunks itself.
-__global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
+__global__ __launch_bounds__(kPlaceThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
                                                                const int32_t *__restrict__ totals) {
     extern __shared__ __align__(16) uint64_t lds[];
-    __shared__ uint64_t scan_tmp[kRouteThreads / 64];
+    __shared__ uint64_t scan_tmp[kPlaceThreads / 64];
     __shared__ uint32_t first[64];
     const int E = a.E;
     uint64_t *mask = lds;                       // [E]
@@ -863,7 +885,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
     const int nt = (int)(a.T - t0 < a.chunk ? a.T - t0 : a.chunk);
     // exclusive sums over the experts: all their rows, and (high half) this chunk's predecessors' rows
     uint64_t run = 0;
-    for (int e0 = 0; e0 < E; e0 += kRouteThreads) {
+    for (int e0 = 0; e0 < E; e0 += kPlaceThreads) {
         const int e = e0 + threadIdx.x;
         uint32_t all = 0, prev = 0;
         if (e < E) {
@@ -881,7 +903,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
             }
         }
         uint64_t sum;
-        const uint64_t pre = run + block_excl_scan<kRouteThreads>((uint64_t)prev << 32 | all, scan_tmp, sum);
+        const uint64_t pre = run + block_excl_scan<kPlaceThreads>((uint64_t)prev << 32 | all, scan_tmp, sum);
         run += sum;
         if (e < E) {
             base[e] = (int32_t)((uint32_t)pre + prev);
@@ -892,23 +914,24 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_place(RouteArgs a, cons
     if (c == 0 && threadIdx.x == 0) a.offsets[E] = total;
     __syncthreads();
     // slots without an expert in the chunks before: all of theirs less the used ones
-    place_chunk(a, t0, nt, mask, base, (int32_t)(total + t0 * a.k - used_all), first);
+    place_chunk<kPlaceThreads>(a, t0, nt, mask, base, (int32_t)(total + t0 * a.k - used_all), first);
 }
 
 // dlogits of one row from the chosen slots' gradients: with a = w / scale,
 //   softmax:                s_i * (scale * g_i [chosen] - sum scale * g_j * s_j)
 //   softmax, renormalised:  scale * a_i * (g_i - sum g_j * a_j) at the chosen
 //   sigmoid:                w_i * (1 - s_i) * g_i at the chosen (renormalised: g_i - sum g_j * a_j)
+constexpr int kGradThreads = 512;
 template <typename T, int L, int V>
-__global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteArgs a, const float *__restrict__ dweights,
+__global__ __launch_bounds__(kGradThreads) void k_route_grad(RouteArgs a, const float *__restrict__ dweights,
                                                               T *__restrict__ dlogits) {
     extern __shared__ __align__(16) uint64_t lds[];
     const int E = a.E, k = a.k;
     const int lane = threadIdx.x & (L - 1), seg = threadIdx.x / L;
     float *d = (float *)lds + (size_t)seg * (L * V);
     const bool full = a.score == 0 && !a.renorm;
-    for (int64_t i0 = (int64_t)blockIdx.x * (kRouteThreads / L); i0 < a.T;
-         i0 += (int64_t)gridDim.x * (kRouteThreads / L)) {
+    for (int64_t i0 = (int64_t)blockIdx.x * (kGradThreads / L); i0 < a.T;
+         i0 += (int64_t)gridDim.x * (kGradThreads / L)) {
         const int64_t t = i0 + seg;
         const bool row = t < a.T;
         const int64_t tt = row ? t : 0;
@@ -1129,16 +1152,23 @@ hipError_t by_type(int32_t dtype, F f) {
     return hipGetLastError();
 }
 
-// lanes and values per lane of a row of E experts
+// Lanes and values per lane of a row of E experts.  Up to 64 experts and many rows: 4 lanes, whose own
+// sorting networks do more of the work (123580 rows, 36 experts in groups, with gradient: 71 -> 50 us);
+// few rows rather take 16 for their latency.
 template <typename F>
-void by_width(int E, F f) {
-    if (E <= 16) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-    else if (E <= 32) f(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
-    else if (E <= 64) f(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
-    else if (E <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
-    else if (E <= 256) f(std::integral_constant<int, 16>(), std::integral_constant<int, 16>());
-    else if (E <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
-    else f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+void by_width(int E, int64_t T, F f) {
+    using std::integral_constant;
+    if (E <= 64 && T > 8192) {
+        if (E <= 16) f(integral_constant<int, 4>(), integral_constant<int, 4>());
+        else if (E <= 32) f(integral_constant<int, 4>(), integral_constant<int, 8>());
+        else f(integral_constant<int, 4>(), integral_constant<int, 16>());
+    } else if (E <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else if (E <= 32) f(integral_constant<int, 16>(), integral_constant<int, 2>());
+    else if (E <= 64) f(integral_constant<int, 16>(), integral_constant<int, 4>());
+    else if (E <= 128) f(integral_constant<int, 16>(), integral_constant<int, 8>());
+    else if (E <= 256) f(integral_constant<int, 16>(), integral_constant<int, 16>());
+    else if (E <= 512) f(integral_constant<int, 64>(), integral_constant<int, 8>());
+    else f(integral_constant<int, 64>(), integral_constant<int, 16>());
 }
 
 }  // namespace
@@ -1217,18 +1247,19 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
     const int64_t chunks = route_chunks(a.T, a.E);
     const int S = a.E / a.groups;
     hipError_t err = hipSuccess;
-    by_width(a.E, [&](auto L, auto V) {
+    by_width(a.E, a.T, [&](auto L, auto V) {
+        constexpr int kThreads = decltype(L)::value == 4 ? 256 : 512;
         // masks; the bases (one chunk); the groups' keys and, for groups of no power of two, the values of
         // every row at once; or a row's values and its groups' in 64 bits for every wave
-        const size_t rows = kRouteThreads / decltype(L)::value, E = a.E, G = a.groups;
+        const size_t rows = kThreads / decltype(L)::value, E = a.E, G = a.groups;
         size_t room = 4 * E;
-        if (G > 1) room = std::max(std::max(room, kRouteThreads / 64 * 8 * (E + G)), rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
+        if (G > 1) room = std::max(std::max(room, kThreads / 64 * 8 * (E + G)), rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
         const size_t lds = 8 * ((E + 1) / 2 * 2) + room;
         auto go = [&](auto KP) {
-            const auto kern = k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value>;
+            const auto kern = k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value, kThreads>;
             if (lds > 64 * 1024)
                 err = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (err == hipSuccess) hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kRouteThreads), lds, s, a);
+            if (err == hipSuccess) hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kThreads), lds, s, a);
         };
         if (a.k <= 4) go(std::integral_constant<int, 4>());
         else if (a.k <= 8) go(std::integral_constant<int, 8>());
@@ -1242,7 +1273,7 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
     if (sums)
         hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 7) / 8)), dim3(1024), 0, s, a.mask, a.before, a.totals,
                            chunks, a.E);
-    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kRouteThreads), 12 * (size_t)a.E, s, a,
+    hipLaunchKernelGGL(k_route_place, dim3((unsigned)chunks), dim3(kPlaceThreads), 12 * (size_t)a.E, s, a,
                        sums ? a.before : nullptr, a.totals);
     return hipGetLastError();
 }
@@ -1251,11 +1282,13 @@ hipError_t launch_route_grad(const RouteArgs &a, const float *dweights, void *dl
     if (a.T <= 0) return hipSuccess;
     return by_type(a.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_width(a.E, [&](auto L, auto V) {
-            const int64_t blocks = (a.T + kRouteThreads / L - 1) / (kRouteThreads / L);
-            hipLaunchKernelGGL((k_route_grad<T, decltype(L)::value, decltype(V)::value>),
-                               dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kRouteThreads),
-                               4 * (size_t)kRouteThreads * V, s, a, dweights, (T *)dlogits);
+        by_width(a.E, 0, [&](auto L, auto V) {
+            if constexpr (decltype(L)::value >= 16) {       // (a lane for each of up to 16 slots)
+                const int64_t blocks = (a.T + kGradThreads / L - 1) / (kGradThreads / L);
+                hipLaunchKernelGGL((k_route_grad<T, decltype(L)::value, decltype(V)::value>),
+                                   dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kGradThreads),
+                                   4 * (size_t)kGradThreads * V, s, a, dweights, (T *)dlogits);
+            }
         });
     });
 }

@@ -197,6 +197,22 @@ def test_route_order_of_many_rows(T):
     check_route(rnd(T, T, 12), 3, valid=torch.rand(T, generator=torch.Generator().manual_seed(1)).to(dev()) < 0.7)
 
 
+@pytest.mark.parametrize("E,k,kw", [
+    (64, 8, {}), (60, 4, dict(renormalise=False)), (33, 16, dict(score="sigmoid", bias=True)), (30, 3, dict(groups=5, top_groups=2)),
+    (32, 8, dict(groups=8, top_groups=5, group_sum=2)), (64, 6, dict(groups=64, top_groups=10, group_sum=2, bias=True)),
+    (36, 1, dict(groups=4, top_groups=3, group_sum=2, score="sigmoid")), (16, 16, {}), (9, 2, dict(bias=True)), (5, 5, {}), (1, 1, {})],
+    ids=str)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_route_of_many_rows_over_few_experts(E, k, kw, dtype):
+    T, kw = 8300, dict(kw)
+    if kw.pop("bias", False):
+        kw["bias"] = rnd(4, E, scale=0.1)
+    l = rnd(T + E, T, E, dtype=dtype, scale=2.0)
+    g = torch.Generator().manual_seed(E)
+    l = l.masked_fill(((torch.rand(T, 1, generator=g) < 0.1) & (torch.rand(T, E, generator=g) < 0.6)).to(dev()), float("-inf"))
+    check_route(l, k, valid=(torch.rand(T, generator=g) < 0.9).to(dev()), **kw)
+
+
 def test_route_of_a_million_rows():
     # more rows than one workgroup's counts can hold: the order is checked by its properties
     T, E, k = 1 << 20, 20, 2
