@@ -544,7 +544,7 @@ __device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i
 // nearer than the keys' and the scores' error is left to choose64 after the others.  Weights come last,
 // KP threads a row.
 template <int L, int V, int KP, int kThreads>
-__global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
+__global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a) {
     extern __shared__ __align__(16) uint64_t lds[];
     __shared__ uint32_t scan_tmp[kThreads / 64], first[64];
     __shared__ unsigned long long odd_rows, nan_rows;
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
             constexpr float kSteps = (float)((1 << (32 - kIndex)) - 8);
             const float scale = by_logit ? kSteps / 16.f : kSteps / 2.f;
             odd |= !(fabsf(top) < 1e6f) && top > -INFINITY;
-            eps = 2.f * scale * (eps > 0.f ? eps + 0x1p-23f * fmaxf(fabsf(top), 1.f) : 0.f) + 4.f;
+            eps = fminf(2.f * scale * (eps > 0.f ? eps + 0x1p-23f * fmaxf(fabsf(top), 1.f) : 0.f) + 5.f, 0x1p30f);
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 uint32_t q;
@@ -743,15 +743,16 @@ __global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
         }
         uint32_t top[KP];
         seg_top<L, V, KP>(key, lane * V, top);
+        const uint32_t near = (uint32_t)eps;        // keys of less distance do not tell the order
+        uint32_t pairs = 0, last = 0;               // bit j: choices j - 1 and j are near; the last choice
+        bool edge = false;                          // the best key that was not chosen is near the last
         if (!exact) {
-            // neighbours nearer than eps, or one at the floor; then the best key that was not chosen
-            uint32_t last = 0;
 #pragma unroll
             for (int j = 0; j < KP; j++) {
                 const uint32_t q = top[j] >> kIndex;
                 if (j < k) {
-                    if (j) odd |= (float)((last >> kIndex) - q) < eps;
-                    odd |= q == 0;
+                    if (j) pairs |= (last >> kIndex) - q < near ? 1u << j : 0u;
+                    odd |= q == 0;                  // at the floor, or no expert at all
                     last = top[j];
                 }
             }
@@ -763,11 +764,11 @@ __global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
                 rest = x > rest ? x : rest;
             }
             rest = seg_reduce<L>(rest, Max());
-            odd |= (float)((last >> kIndex) - (rest >> kIndex)) < eps;
+            edge = (last >> kIndex) - (rest >> kIndex) < near;
         }
         odd = seg_reduce<L>((int)odd, Or()) != 0 && on;
         if (row && lane == 0) {
-            // (a key at the floor may be of no expert at all: choose64 writes the odd rows' experts)
+            // (odd rows' experts are choose64's)
             const uint32_t field = exact ? kExactMask : kIndexMask;
             uint32_t pair[KP / 2];
 #pragma unroll
@@ -778,8 +779,37 @@ __global__ __launch_bounds__(kThreads, 4) void k_route(RouteArgs a) {
             }
             __builtin_memcpy(__builtin_assume_aligned(chosen + i * KP, KP >= 8 ? 16 : 8), pair, sizeof(pair));
             if (exps) stat[i] = make_float2(m, sum);
-            if (odd) atomicOr(&odd_rows, 1ull << i);
         }
+        if (__any((pairs || edge) && on && !odd)) {
+            // Near ones of the same logit and bias are equal, and stand in the order of their indexes already
+            // (16-bit logits and biases that move in steps make many of them); others make the row odd.
+            wave_lds_sync();
+            if (!on || odd) pairs = 0, edge = false;
+            auto same = [&](int e, int f) {
+                bool eq = one_logit(a, t, e) == one_logit(a, t, f);
+                if (a.bias) eq = eq && bias[(e % V / kVec * L + e / V) * kVec + e % V % kVec] ==
+                                           bias[(f % V / kVec * L + f / V) * kVec + f % V % kVec];
+                return eq;
+            };
+            for (; pairs; pairs &= pairs - 1) {
+                const int j = __builtin_ctz(pairs);
+                if (!same(chosen[i * KP + j - 1], chosen[i * KP + j])) { odd = true; break; }
+            }
+            if (edge && !odd) {
+                uint32_t close = 0;
+                const uint32_t below = last + lane * V;
+#pragma unroll
+                for (int v = 0; v < V; v++)
+                    close |= key[v] < below && (last >> kIndex) - (key[v] >> kIndex) < near ? 1u << v : 0u;
+                const int e = chosen[i * KP + k - 1];
+                for (; close; close &= close - 1) {
+                    const int f = lane * V + __builtin_ctz(close);
+                    if (f < E && !same(e, f)) { odd = true; break; }
+                }
+            }
+            odd = seg_reduce<L>((int)odd, Or()) != 0;
+        }
+        if (odd && lane == 0) atomicOr(&odd_rows, 1ull << i);
     }
     __syncthreads();
     // the rows left, a wave each
