@@ -267,7 +267,7 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
  *   has the place pos[s] in the order by (expert, t); slots without an expert come after
  *   offsets[experts], in their own order; src is the inverse of pos.
  *   slopes (NULL: not wanted) gets 1 - s of the chosen experts for the gradient of PSS_SIGMOID.
- * experts <= 1024, k <= 16, groups <= 64, tokens * k < 2^31.  ws: pss_route_workspace bytes, used by
+ * experts <= 1024, k <= 16, groups <= 64, tokens < 2^28, tokens * k < 2^31.  ws: pss_route_workspace bytes, used by
  * this call alone while it runs.  Results do not depend on timing: no order of atomics enters. */
 #define PSS_SOFTMAX 0
 #define PSS_SIGMOID 1

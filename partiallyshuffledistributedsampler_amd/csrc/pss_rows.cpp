@@ -161,7 +161,8 @@ static int route_args(RouteArgs *a, const void *logits, int64_t ld, int64_t toke
         return set_error(PSS_EINVAL, "route: tokens >= 0 and 1 <= k <= experts");
     if (experts > kRouteMaxE || k > kRouteMaxK)
         return set_error(PSS_ENOTSUP, "route: at most 1024 experts, 16 of them for a row");
-    if (tokens * k >= ((int64_t)1 << 31)) return set_error(PSS_ENOTSUP, "route: 2^31 slots or more");
+    if (tokens >= (int64_t)1 << 28 || tokens * k >= (int64_t)1 << 31)
+        return set_error(PSS_ENOTSUP, "route: 2^28 rows, or 2^31 slots, or more");
     if (tokens > 0 && !logits) return set_error(PSS_EINVAL, "route: NULL logits");
     if (ld < 0) return set_error(PSS_EINVAL, "the row stride must be >= 0");
     if (score != PSS_SOFTMAX && score != PSS_SIGMOID) return set_error(PSS_EINVAL, "route: score must be PSS_SOFTMAX or PSS_SIGMOID");

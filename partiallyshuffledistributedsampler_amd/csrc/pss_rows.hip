@@ -705,9 +705,9 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
             if (!exact) {
                 least = seg_reduce<L>(least, Min());
                 most = seg_reduce<L>(most, Max());
-                // two scores' errors on either side, the roundings of their sums, and the keys' 64 units
+                // two scores' errors on either side, and of the sums the roundings and the keys' 64 units
                 const float p = group_value(least), q = group_value(most);
-                if (most) odd |= !(p - q > 4.f * eps + 0x1p-17f * fmaxf(fabsf(p), fabsf(q))) && q > -INFINITY;
+                if (most) odd |= !(p - q > 4.f * eps + 0x1.4p-17f * fmaxf(fabsf(p), fabsf(q))) && q > -INFINITY;
             }
             wave_lds_sync();
             const uint32_t g0 = ((uint32_t)(lane * V) * inv) >> 20;
@@ -913,7 +913,8 @@ __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict_
 }
 
 // Places of one chunk's slots: the chunk's masks and sums, one scan over the experts, then a popcount a
-// slot.  Bound by latency: 7.7 us for 65536 x 8 slots, 4 for 16381 x 4.  Without the sums of k_route_scan a workgroup counts all chunks itself.
+// slot.  Bound by latency: 7.7 us for 65536 x 8 slots, 4 for 16381 x 4.  Without the sums of k_route_scan
+// a workgroup counts all chunks itself.
 __global__ __launch_bounds__(kPlaceThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
                                                                const int32_t *__restrict__ totals) {
     extern __shared__ __align__(16) uint64_t lds[];
@@ -1206,11 +1207,11 @@ hipError_t by_type(int32_t dtype, F f) {
 
 // Lanes and values per lane of a row of E experts.  Up to 64 experts and many rows: 4 lanes, whose own
 // sorting networks do more of the work (123580 rows, 36 experts in groups, with gradient: 71 -> 50 us);
-// few rows rather take 16 for their latency.
+// few rows rather take 16 for their latency.  V <= E: a lane past the end reads the row's last V values.
 template <typename F>
 void by_width(int E, int64_t T, F f) {
     using std::integral_constant;
-    if (E <= 64 && T > 8192) {
+    if (E >= 4 && E <= 64 && T > 8192) {
         if (E <= 16) f(integral_constant<int, 4>(), integral_constant<int, 4>());
         else if (E <= 32) f(integral_constant<int, 4>(), integral_constant<int, 8>());
         else f(integral_constant<int, 4>(), integral_constant<int, 16>());
@@ -1307,6 +1308,10 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t s) {
         size_t room = 4 * E;
         if (G > 1) room = std::max(std::max(room, kThreads / 64 * 8 * (E + G)), rows * 4 * ((G + 3) / 4 * 4 + (S & (S - 1) ? (size_t)(L * V) : 0)));
         const size_t lds = 8 * ((E + 1) / 2 * 2) + room;
+        if (decltype(V)::value > a.E || decltype(L)::value * decltype(V)::value < a.E) {
+            err = hipErrorInvalidValue;     // (no width does)
+            return;
+        }
         auto go = [&](auto KP) {
             const auto kern = k_route<decltype(L)::value, decltype(V)::value, decltype(KP)::value, kThreads>;
             if (lds > 64 * 1024)

@@ -108,7 +108,7 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
 
     The best choice first, ties to the lower index.  A logit of -inf masks the expert; a row with
     fewer than k left has experts -1 and weights 0 in its last slots.  Gradients flow from
-    Routing.weights to the logits.  E <= 1024, k <= 16, groups <= 64, T * k < 2^31."""
+    Routing.weights to the logits.  E <= 1024, k <= 16, groups <= 64, T < 2^28, T * k < 2^31."""
     if score not in SCORES:
         raise ValueError("score must be 'softmax' or 'sigmoid', got %r" % (score,))
     return Routing(*_c.route(logits, k, SCORES[score], bias, valid, groups, top_groups, group_sum, bool(renormalise), scale))

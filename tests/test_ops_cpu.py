@@ -205,7 +205,7 @@ def _route_rc(tokens=0, experts=8, k=2, dtype=0, score=0, groups=1, top_groups=1
     (dict(groups=4, top_groups=0), 1), (dict(groups=8, top_groups=1), 1), (dict(group_sum=3), 1), (dict(scale=0.0), 1),
     (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1), (dict(ld=-1), 1), (dict(tokens=4), 1),
     (dict(offsets=None), 1), (dict(experts=1025), 3), (dict(experts=64, k=17), 3),
-    (dict(experts=128, groups=128, top_groups=128), 3), (dict(tokens=1 << 30), 3)], ids=str)
+    (dict(experts=128, groups=128, top_groups=128), 3), (dict(tokens=1 << 30), 3), (dict(tokens=1 << 28, k=1), 3)], ids=str)
 def test_route_entry_refuses_on_the_host(bad, code):
     # every pointer is NULL or never dereferenced: the entry returns before any device work
     assert _route_rc(**bad) == code
