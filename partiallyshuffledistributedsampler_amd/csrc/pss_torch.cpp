@@ -23,7 +23,7 @@ using torch::autograd::variable_list;
 // ---- the C entries -------------------------------------------------------------------------------
 #define ENTRIES(F) \
     F(pss_last_error) F(pss_dropout) F(pss_route_workspace) F(pss_route) F(pss_route_grad) F(pss_dispatch) \
-    F(pss_combine) F(pss_combine_grad)
+    F(pss_combine) F(pss_combine_grad) F(pss_gather_dropout)
 struct Entries {
 #define FIELD(name) decltype(&::name) name = nullptr;
     ENTRIES(FIELD)
@@ -167,6 +167,44 @@ Tensor dropout(const Tensor &x, double p, uint64_t key, int64_t row0, const Opt 
         i = ids->reshape({-1}).contiguous();
     }
     return Dropout::apply(x, residual, p, (int64_t)key, row0, opt(i));
+}
+
+// ---- gather with dropout -------------------------------------------------------------------------
+// Rows of device-resident files (IndexEngine.gather with p > 0): `device` is the handle's.
+Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Tensor &data, const Tensor &base_rows_,
+              const Tensor &fpos_, const Tensor &off_, const Opt &out_, double p, uint64_t key, int64_t row0,
+              const Opt &ids_) {
+    check_p(p);
+    TORCH_CHECK_TYPE(dtype_of(data) >= 0, "gather with dropout needs float32, bfloat16 or float16 data, got ",
+                     data.scalar_type());
+    TORCH_CHECK_VALUE(data.device() == device && data.is_contiguous() && data.dim() > 0,
+                      "gather: data must be contiguous rows on the engine's device");
+    const Tensor fpos = fpos_.reshape({-1}).contiguous(), off = off_.reshape({-1}).to(at::kInt).contiguous();
+    const Tensor base = base_rows_.to(device, at::kLong).contiguous();
+    const int64_t n = fpos.numel(), values = data.size(0) ? data.numel() / data.size(0) : 0;
+    TORCH_CHECK_VALUE(fpos.scalar_type() == at::kInt && fpos.device() == device && off.device() == device,
+                      "gather: file_pos and offset must be int32 on the engine's device");
+    TORCH_CHECK_VALUE(off.numel() == n && base.numel() >= files,
+                      "gather: file_pos and offset must be of one length, base_rows must have an entry for each of the ",
+                      files, " files");
+    Tensor out = get(out_), ids = get(ids_);
+    if (out.defined()) {
+        TORCH_CHECK_VALUE(out.is_contiguous() && out.scalar_type() == data.scalar_type() && out.device() == device &&
+                              out.numel() >= n * values,
+                          "gather: out must be contiguous, of the data's dtype, on the engine's device");
+    } else {
+        auto sizes = data.sizes().vec();
+        sizes[0] = n;
+        out = at::empty(sizes, data.options());
+    }
+    check_ids(ids, n, data);
+    if (ids.defined()) ids = ids.reshape({-1}).contiguous();
+    check(lib.pss_gather_dropout((pss_sampler *)handle, data.const_data_ptr(), dtype_of(data), values,
+                                 base.const_data_ptr<int64_t>(), fpos.const_data_ptr<int32_t>(),
+                                 off.const_data_ptr<int32_t>(), n, p, key, row0, ids_ptr(ids), ids_n(ids),
+                                 out.data_ptr(), data.is_cpu() ? nullptr : stream_of(data)),
+          "pss_gather_dropout");
+    return out;
 }
 
 // ---- routing -------------------------------------------------------------------------------------
@@ -363,6 +401,7 @@ Tensor combine(const Tensor &y, const Tensor &weights, const Tensor &experts, co
 PYBIND11_MODULE(_pss_torch, m) {
     m.def("bind", &bind);
     m.def("dropout", &dropout);
+    m.def("gather", &gather);
     m.def("route", &route);
     m.def("dispatch", &dispatch);
     m.def("combine", &combine);

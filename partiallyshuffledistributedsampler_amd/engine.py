@@ -167,6 +167,9 @@ class IndexEngine:
         (file_pos, offset) pairs, in their order (the on-GPU form of V1:243-248).
         p > 0: the rows (float32, bfloat16 or float16) with dropout, in the same pass
         (pss_gather_dropout) -- exactly ops.dropout(rows flattened to [n, values], p, key, rows)."""
+        if p:
+            from . import ops
+            return ops.gather(self, data, base_rows, fpos, off, out, stream, p, key, rows)
         d = self._dev()
         if fpos.dim() != 1 or not fpos.is_contiguous():
             fpos = fpos.reshape(-1).contiguous()
@@ -179,29 +182,6 @@ class IndexEngine:
         row_bytes = math.prod(data.shape[1:]) * data.element_size() if data.dim() > 0 and data.shape[0] else 0
         if out is None:
             out = torch.empty((n,) + tuple(data.shape[1:]), dtype=data.dtype, device=d)
-        if p:
-            from .ops import DTYPES, _row_ids
-            if data.dtype not in DTYPES:
-                raise TypeError("gather with dropout needs float32, bfloat16 or float16 data, got %s" % data.dtype)
-            if not (out.is_contiguous() and out.dtype == data.dtype and out.device == d
-                    and out.numel() >= n * (row_bytes // data.element_size())):
-                raise ValueError("gather: out must be contiguous, of the data's dtype, on the engine's device")
-            if not 0.0 <= p <= 1.0:
-                raise ValueError("p must be in [0, 1], got %r" % p)
-            if off.numel() != n or base_rows.numel() < self.num_files:
-                raise ValueError("gather: file_pos and offset must be of one length, base_rows must have an "
-                                 "entry for each of the %d files" % self.num_files)
-            row0, ids = _row_ids(rows)
-            if ids is not None:
-                if ids.dtype != torch.int64 or ids.device != d or ids.numel() not in (1, n):
-                    raise ValueError("rows must be an int, or an int64 tensor of one id or %d ids on the "
-                                     "engine's device" % n)
-                ids = ids.reshape(-1).contiguous()
-            _lib.call("pss_gather_dropout", self._h, data.data_ptr(), DTYPES[data.dtype],
-                      row_bytes // data.element_size(), base_rows.data_ptr(), fpos.data_ptr(), off.data_ptr(), n,
-                      float(p), int(key) & 0xFFFFFFFFFFFFFFFF, row0, None if ids is None else ids.data_ptr(),
-                      0 if ids is None else ids.numel(), out.data_ptr(), _stream_ptr(stream, d))
-            return out
         _lib.call("pss_gather", self._h, ctypes.c_void_p(data.data_ptr()), row_bytes,
                   ctypes.c_void_p(base_rows.data_ptr()), ctypes.c_void_p(fpos.data_ptr()),
                   ctypes.c_void_p(off.data_ptr()), n, ctypes.c_void_p(out.data_ptr()),

@@ -27,11 +27,10 @@ import torch
 
 from . import _lib
 
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 SCORES = {"softmax": 0, "sigmoid": 1}
 _MASK64 = (1 << 64) - 1
 _ENTRIES = ("pss_last_error", "pss_dropout", "pss_route_workspace", "pss_route", "pss_route_grad",
-            "pss_dispatch", "pss_combine", "pss_combine_grad")
+            "pss_dispatch", "pss_combine", "pss_combine_grad", "pss_gather_dropout")
 
 
 def _load():
@@ -92,6 +91,16 @@ def dropout(x, p, key, rows=0, residual=None):
     leading dimensions of x are rows, in order."""
     row0, ids = _row_ids(rows)
     return _c.dropout(x, p, int(key) & _MASK64, row0, ids, residual)
+
+
+def gather(engine, data, base_rows, fpos, off, out=None, stream=None, p=0.0, key=0, rows=0):
+    """IndexEngine.gather(..., p, key, rows): rows of device-resident files with dropout."""
+    if stream is not None and not engine.cpu:
+        with torch.cuda.stream(stream):     # (what the call allocates belongs to that stream, too)
+            return gather(engine, data, base_rows, fpos, off, out, None, p, key, rows)
+    row0, ids = _row_ids(rows)
+    return _c.gather(engine._h.value if engine._h else 0, engine._dev(), engine.num_files, data, base_rows, fpos, off,
+                     out, p, int(key) & _MASK64, row0, ids)
 
 
 def route(logits, k, *, score="softmax", bias=None, groups=1, top_groups=1, group_sum=1, renormalise=True, scale=1.0,

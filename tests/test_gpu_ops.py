@@ -101,6 +101,11 @@ def test_gather_with_dropout(dtype, shape):
         got = eng.gather(data, base, fpos, off, p=p, key=42, rows=1 << 33)
         want = ops.dropout(plain.reshape(total, -1), p, 42, rows=1 << 33).reshape(plain.shape)
         assert torch.equal(got, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = eng.gather(data, base, fpos[:, ::2], off[:, ::2].long(), p=0.3, key=42, stream=side)
+    side.synchronize()
+    assert torch.equal(got.reshape(len(got), -1), ops.dropout(plain.reshape(total, -1)[::2], 0.3, 42))
     out = torch.empty_like(plain)
     assert eng.gather(data, base, fpos[:, :7], off[:, :7], out=out[:7], p=0.3, key=42).data_ptr() == out.data_ptr()
     assert torch.equal(out[:7], ops.dropout(plain.reshape(total, -1)[:7], 0.3, 42).reshape(7, *shape))
