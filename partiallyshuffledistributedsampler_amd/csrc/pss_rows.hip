@@ -37,21 +37,20 @@ __device__ __forceinline__ __bf16 at(__bf16 v, int) { return v; }
 __device__ __forceinline__ _Float16 at(_Float16 v, int) { return v; }
 template <typename V> __device__ __forceinline__ auto at(const V &v, int i) { return v[i]; }
 
-// NT: past the caches (nontemporal)
-template <bool NT = false, typename T, int N>
-__device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N], float fill = 0.f) {
+template <typename T, int N>
+__device__ __forceinline__ void load(const T *p, int64_t left, float (&v)[N]) {
     if (left >= N) {
         typedef typename Pack<T, N>::V V;
-        const V a = NT ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
+        const V a = *(const V *)p;
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = Value<T>::up(at(a, i));
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < left ? Value<T>::up(p[i]) : fill;
+        for (int i = 0; i < N; i++) v[i] = i < left ? Value<T>::up(p[i]) : 0.f;
     }
 }
 
-template <bool NT = false, typename T, int N>
+template <typename T, int N>
 __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
     if (left >= N) {
         if constexpr (N == 1) {
@@ -60,13 +59,72 @@ __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
             typename Pack<T, N>::V a;
 #pragma unroll
             for (int i = 0; i < N; i++) a[i] = Value<T>::down(v[i]);
-            if (NT) __builtin_nontemporal_store(a, (typename Pack<T, N>::V *)p);
-            else *(typename Pack<T, N>::V *)p = a;
+            *(typename Pack<T, N>::V *)p = a;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
             if (i < left) p[i] = Value<T>::down(v[i]);
+    }
+}
+
+// Eight values of a row of D, from column c (a multiple of 8) on, 0 past the end.  A lane at the end reads
+// the row's last eight and shifts them down: every lane makes the same wide load and several rows' loads
+// stay on their way, where a branch that reads the end value by value waits for each (combine of 8 rows
+// of 4095 bf16 of 8194 tokens: 169 -> 113 us; dropout of 16386 x 8191 bf16: 156 -> 122).  raw8 is the load
+// (NT: nontemporal, past the caches), open8 the rest.  WHOLE (gather and dropout): D % 8 is 0, and
+// no branch stands between the load and the Philox block (gather of 65536 x 2048 bf16: 162 -> 99).
+template <bool NT = false, bool WHOLE = false, typename T>
+__device__ __forceinline__ typename Pack<T, 8>::V raw8(const T *row, int64_t c, int64_t D) {
+    typedef typename Pack<T, 8>::V V;
+    if (WHOLE) return NT ? __builtin_nontemporal_load((const V *)(row + c)) : *(const V *)(row + c);
+    if (D >= 8) {
+        const V *p = (const V *)(row + (c <= D - 8 ? c : D - 8));
+        return NT ? __builtin_nontemporal_load(p) : *p;
+    }
+    V a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = i < D ? row[i] : (T)0.f;
+    return a;
+}
+template <typename T, bool WHOLE = false, typename V>
+__device__ __forceinline__ void open8(const V &a, int64_t c, int64_t D, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = Value<T>::up(a[i]);
+    if (!WHOLE && D > 8 && D % 8) {
+        const int by = c > D - 8 ? (int)(c - (D - 8)) : 0;
+#pragma unroll
+        for (int s = 1; s < 8; s *= 2)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = !(by & s) ? v[i] : i + s < 8 ? v[i + s] : 0.f;
+    }
+}
+template <bool NT = false, bool WHOLE = false, typename T>
+__device__ __forceinline__ void load8(const T *row, int64_t c, int64_t D, float (&v)[8]) {
+    open8<T, WHOLE>(raw8<NT, WHOLE>(row, c, D), c, D, v);
+}
+// and the values back: what is left of a row in pieces of 4, 2 and 1
+template <bool NT = false, bool WHOLE = false, typename T>
+__device__ __forceinline__ void store8(T *row, int64_t c, int64_t D, const float (&v)[8]) {
+    typename Pack<T, 8>::V a;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a[i] = Value<T>::down(v[i]);
+    T *p = row + c;
+    const int left = WHOLE || D - c >= 8 ? 8 : (int)(D - c);
+    if (left == 8) {
+        if (NT) __builtin_nontemporal_store(a, (typename Pack<T, 8>::V *)p);
+        else *(typename Pack<T, 8>::V *)p = a;
+    } else {
+        if (left & 4) {
+            *(typename Pack<T, 4>::V *)p = __builtin_shufflevector(a, a, 0, 1, 2, 3);
+            p += 4;
+        }
+        const auto b = left & 4 ? __builtin_shufflevector(a, a, 4, 5, 6, 6) : __builtin_shufflevector(a, a, 0, 1, 2, 2);
+        if (left & 2) {
+            *(typename Pack<T, 2>::V *)p = __builtin_shufflevector(b, b, 0, 1);
+            p += 2;
+        }
+        if (left & 1) *p = left & 2 ? b[2] : b[0];
     }
 }
 
@@ -98,9 +156,9 @@ __device__ __forceinline__ void drop8(const Drop &d, const Draw &u, float (&v)[8
 // y = dropout(x) (+ residual).  Bound by memory: a value is read (twice with a residual) and written, and
 // 20 32 x 32-bit products per 8 values hide behind that.  One thread per block of 8 columns, over rows and
 // blocks as one range, so that odd widths leave no lanes idle; (row, block) are stepped, not divided.
-// 16384 x 8192 bf16: 132 us with a residual (6.1 TB/s), 93 without (5.7); 4093 x 1537 fp32, from the
-// Infinity Cache: 13 and 11.
-template <typename T, bool RES, bool NT>
+// 16384 x 8192 bf16: 133 us with a residual (6.1 TB/s), 91 without (5.9); x 8191, whose rows start at
+// any 2 bytes, 171 and 115; 4093 x 1537 fp32, from the Infinity Cache: 14 and 10.
+template <typename T, bool RES, bool NT, bool WHOLE>
 __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,
                                                  int64_t ldr, T *__restrict__ y, int64_t rows, int64_t cols,
                                                  uint32_t nb, Drop d) {
@@ -111,18 +169,20 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
     const int64_t drow = step / nb;
     const uint32_t db = (uint32_t)(step - drow * nb);
     while (row < rows) {
-        const int64_t c = (int64_t)b * 8, left = cols - c;
+        const int64_t c = (int64_t)b * 8;
         float v[8];
-        load<NT>(x + row * ldx + c, left, v);
+        load8<NT, WHOLE>(x + row * ldx, c, cols, v);
         float r[8];
-        if (RES) load<NT>(res + row * ldr + c, left, r);
+        Draw dr;
+        if (d.drop) dr = draw8(d, drop_row(d, row), b);
+        if (RES) load8<NT, WHOLE>(res + row * ldr, c, cols, r);     // after the block: 140 -> 133 us
         if (d.drop) {
-            drop8<RES>(d, draw8(d, drop_row(d, row), b), v, r);
+            drop8<RES>(d, dr, v, r);
         } else if (RES) {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] += r[i];
         }
-        store<NT>(y + row * cols + c, left, v);
+        store8<NT, WHOLE>(y + row * cols, c, cols, v);
         row += drow;
         b += db;
         if (b >= nb) { b -= nb; row++; }
@@ -130,7 +190,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_
 }
 
 // ---- routing -------------------------------------------------------------------------------------
-// The lanes of a segment (4, 8, 16 or 64 of a wave) share one row; reductions stay inside the segment.  Step
+// The lanes of a segment (4, 8, 16, 32 or 64 of a wave) share one row; reductions stay inside the segment.  Step
 // i joins lanes that hold the same after the steps before: 1 and 2 apart, then the halves of 8 and 16
 // mirrored (DPP, no LDS), then 16 and 32 apart.
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_mov(uint32_t x) {
@@ -165,10 +225,8 @@ __device__ __forceinline__ T seg_reduce(T v, F f) {
     v = f(v, partner<1>(v));
     if constexpr (L >= 8) v = f(v, partner<2>(v));
     if constexpr (L >= 16) v = f(v, partner<3>(v));
-    if constexpr (L == 64) {
-        v = f(v, partner<4>(v));
-        v = f(v, partner<5>(v));
-    }
+    if constexpr (L >= 32) v = f(v, partner<4>(v));
+    if constexpr (L == 64) v = f(v, partner<5>(v));
     return v;
 }
 struct Max { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
@@ -1023,7 +1081,7 @@ __global__ __launch_bounds__(kGradThreads) void k_route_grad(RouteArgs a, const 
 }
 
 // ---- rows moved: gather, dispatch, combine -------------------------------------------------------
-// L lanes of a 256-thread workgroup share one row (16, 64 or all 256), eight columns a lane and step;
+// L lanes of a 256-thread workgroup share one row (16, 32, 64 or all 256), eight columns a lane and step;
 // gridDim.y workgroups share its columns where there are few rows.  A place outside the T * k rows (a
 // plan that route did not make) is taken as a slot without an expert, and nothing is written there.
 template <int L>
@@ -1034,25 +1092,45 @@ __device__ __forceinline__ int64_t first_row() {
 template <int L> __device__ __forceinline__ int64_t row_step() { return (int64_t)gridDim.x * (256 / L); }
 template <int L> __device__ __forceinline__ int64_t first_col() { return ((int64_t)blockIdx.y * L + threadIdx.x % L) * 8; }
 template <int L> __device__ __forceinline__ int64_t col_step() { return (int64_t)gridDim.y * L * 8; }
-
+// f(row, column of its eight values) over all of them; L = 0: a thread per eight values over rows and
+// columns as one range, so that no lane of a narrow row is idle ((row, block) are stepped, not divided)
+template <int L, typename F>
+__device__ __forceinline__ void each8(int64_t rows, int64_t cols, F f) {
+    if constexpr (L) {
+        for (int64_t r = first_row<L>(); r < rows; r += row_step<L>())
+            for (int64_t c = first_col<L>(); c < cols; c += col_step<L>()) f(r, c);
+    } else {
+        const uint32_t nb = (uint32_t)((cols + 7) / 8), at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+        const uint32_t dr = step / nb, db = step - dr * nb;
+        int64_t r = at / nb;
+        uint32_t b = at % nb;
+        while (r < rows) {
+            f(r, (int64_t)b * 8);
+            r += dr;
+            b += db;
+            if (b >= nb) { b -= nb; r++; }
+        }
+    }
+}
 
 // out[r] = dropout(row base[order[f_r]] + off_r of the data).  Bound by memory, a row's index loads first:
 // they are the same for the lanes of a row (scalar loads), and rows of other waves cover them.
-// 65536 rows of 2048 bf16: 99 us (5.4 TB/s).
-template <typename T, int L, bool NT>
+// 65536 rows of 2048 bf16: 95 us (5.6 TB/s), of 2047 123.
+template <typename T, int L, bool NT, bool WHOLE>
 __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data, T *__restrict__ out, int64_t rows,
                                                      int64_t cols, Drop d, RowGather g) {
-    for (int64_t r = first_row<L>(); r < rows; r += row_step<L>()) {
+    each8<L>(rows, cols, [&](int64_t r, int64_t c) {
         const int32_t f = g.fpos[r] < 0 ? -1 - g.fpos[r] : g.fpos[r];
         const T *x = data + (g.base[g.order[f]] + g.off[r]) * cols;
         const int64_t id = drop_row(d, r);
-        for (int64_t c = first_col<L>(); c < cols; c += col_step<L>()) {
-            float v[8];
-            load<NT>(x + c, cols - c, v);
-            if (d.drop) drop8<false>(d, draw8(d, id, (uint32_t)(c >> 3)), v, v);
-            store<NT>(out + r * cols + c, cols - c, v);
-        }
-    }
+        const auto a = raw8<NT, WHOLE>(x, c, cols);
+        Draw dr;
+        if (d.drop) dr = draw8(d, id, (uint32_t)(c >> 3));      // while the values come
+        float v[8];
+        open8<T, WHOLE>(a, c, cols, v);
+        if (d.drop) drop8<false>(d, dr, v, v);
+        store8<NT, WHOLE>(out + r * cols, c, cols, v);
+    });
 }
 
 // xs[pos[t, j]] = x[t].  Bound by the k writes of a row, which is read once (a gather by place would read
@@ -1060,64 +1138,63 @@ __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data,
 template <typename T, int L>
 __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restrict__ x, int64_t ldx, T *__restrict__ xs) {
     const uint32_t places = (uint32_t)(m.T * m.k);
-    for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
+    each8<L>(m.T, m.D, [&](int64_t t, int64_t c) {
         const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
-        for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
-            float v[8];
-            const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            load(x + t * ldx + c, m.D - c, v);
-            for (int j = 0; j < m.k; j++) {
-                if ((uint32_t)pos[j] >= places) continue;
-                T *to = xs + (int64_t)pos[j] * m.D + c;
-                if (e[j] >= 0) store(to, m.D - c, v);
-                else store(to, m.D - c, zero);
-            }
+        float v[8];
+        const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        load8(x + t * ldx, c, m.D, v);
+        for (int j = 0; j < m.k; j++) {
+            if ((uint32_t)pos[j] >= places) continue;
+            T *to = xs + (int64_t)pos[j] * m.D;
+            if (e[j] >= 0) store8(to, c, m.D, v);
+            else store8(to, c, m.D, zero);
         }
-    }
+    });
 }
 
 // out[t] = residual[t] + dropout(sum of w[t, j] * y[pos[t, j]]), the gradient of k_dispatch without weights
 // and residual.  Bound by the reads of k rows: KU of them are on their way at a time, and the Philox block
-// is computed meanwhile.  16384 x 8 rows of 4096 bf16: 238 us (5.1 TB/s), with residual and dropout 267.  A slot without an expert is read like any other (its place
-// is a row of y) and left out of the sum whatever it holds.
+// is computed meanwhile.  16384 x 8 rows of 4096 bf16: 238 us (5.1 TB/s), with residual and dropout
+// 267; 8194 x 8 of 4095 113 (5.3).  A slot without an expert is read like any other (its place is a row of
+// y) and left out of the sum whatever it holds.
 template <typename T, int L, int KU, bool NT>
 __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict__ y, const float *__restrict__ w,
                                                  const T *__restrict__ res, int64_t ldr, Drop d, T *__restrict__ out) {
     const uint32_t places = (uint32_t)(m.T * m.k);
-    for (int64_t t = first_row<L>(); t < m.T; t += row_step<L>()) {
+    each8<L>(m.T, m.D, [&](int64_t t, int64_t c) {
         const int32_t *e = m.experts + t * m.k, *pos = m.pos + t * m.k;
         const int64_t id = d.drop ? drop_row(d, t) : 0;
-        for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
-            float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (res) load<NT>(res + t * ldr + c, m.D - c, r);
-            Draw dr;
-            for (int j0 = 0; j0 < m.k; j0 += KU) {
-                float v[KU][8];
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (res) load8<NT>(res + t * ldr, c, m.D, r);
+        Draw dr;
+        for (int j0 = 0; j0 < m.k; j0 += KU) {
+            typename Pack<T, 8>::V raw[KU];
 #pragma unroll
-                for (int u = 0; u < KU; u++) {
-                    const int j = j0 + u < m.k ? j0 + u : j0;
-                    const uint32_t at = (uint32_t)pos[j] < places ? (uint32_t)pos[j] : 0u;
-                    load<NT>(y + (int64_t)at * m.D + c, m.D - c, v[u]);
-                }
-                if (d.drop && j0 == 0) dr = draw8(d, id, (uint32_t)(c >> 3));   // while the rows come
-#pragma unroll
-                for (int u = 0; u < KU; u++) {
-                    const int j = j0 + u < m.k ? j0 + u : j0;
-                    const bool on = j0 + u < m.k && e[j] >= 0 && (uint32_t)pos[j] < places;
-                    const float wj = w ? w[t * m.k + j] : 1.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[i] = on ? fmaf(wj, v[u][i], acc[i]) : acc[i];
-                }
+            for (int u = 0; u < KU; u++) {
+                const int j = j0 + u < m.k ? j0 + u : j0;
+                const uint32_t at = (uint32_t)pos[j] < places ? (uint32_t)pos[j] : 0u;
+                raw[u] = raw8<NT>(y + (int64_t)at * m.D, c, m.D);
             }
-            if (d.drop) {
-                drop8<true>(d, dr, acc, r);
-            } else if (res) {
+            if (d.drop && j0 == 0) dr = draw8(d, id, (uint32_t)(c >> 3));   // while the rows come
 #pragma unroll
-                for (int i = 0; i < 8; i++) acc[i] += r[i];
+            for (int u = 0; u < KU; u++) {
+                const int j = j0 + u < m.k ? j0 + u : j0;
+                const bool on = j0 + u < m.k && e[j] >= 0 && (uint32_t)pos[j] < places;
+                const float wj = w ? w[t * m.k + j] : 1.f;
+                float v[8];
+                open8<T>(raw[u], c, m.D, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[i] = on ? fmaf(wj, v[i], acc[i]) : acc[i];
             }
-            store<NT>(out + t * m.D + c, m.D - c, acc);
         }
-    }
+        if (d.drop) {
+            drop8<true>(d, dr, acc, r);
+        } else if (res) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[i] += r[i];
+        }
+        store8<NT>(out + t * m.D, c, m.D, acc);
+    });
 }
 
 // One pass over g = dropout(dout): KU products with rows of y and KU rows of dy at a time.  The lanes
@@ -1148,19 +1225,22 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
         }
         for (int64_t c = first_col<L>(); c < m.D; c += col_step<L>()) {
             float g[8];
-            load(dout + t * ldo + c, m.D - c, g);
+            load8(dout + t * ldo, c, m.D, g);
             if (d.drop) drop8<false>(d, draw8(d, id, (uint32_t)(c >> 3)), g, g);
 #pragma unroll
             for (int j0 = 0; j0 < KM; j0 += KU) {
                 if (j0 >= m.k) break;
                 if (dw) {
-                    float v[KU][8];
+                    typename Pack<T, 8>::V raw[KU];
 #pragma unroll
-                    for (int u = 0; u < KU; u++) load<NT>(y + (int64_t)pos[j0 + u] * m.D + c, m.D - c, v[u]);
+                    for (int u = 0; u < KU; u++) raw[u] = raw8<NT>(y + (int64_t)pos[j0 + u] * m.D, c, m.D);
 #pragma unroll
-                    for (int u = 0; u < KU; u++)
+                    for (int u = 0; u < KU; u++) {
+                        float v[8];
+                        open8<T>(raw[u], c, m.D, v);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) dot[j0 + u] = fmaf(g[i], v[u][i], dot[j0 + u]);
+                        for (int i = 0; i < 8; i++) dot[j0 + u] = fmaf(g[i], v[i], dot[j0 + u]);
+                    }
                 }
                 if (dy) {
 #pragma unroll
@@ -1170,7 +1250,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t 
                         float o[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++) o[i] = on[j0 + u] ? wt[j0 + u] * g[i] : 0.f;
-                        store(dy + (int64_t)pos[j0 + u] * m.D + c, m.D - c, o);
+                        store8(dy + (int64_t)pos[j0 + u] * m.D, c, m.D, o);
                     }
                 }
             }
@@ -1228,10 +1308,10 @@ void by_width(int E, int64_t T, F f) {
 
 // Whether a pass over so many bytes goes past the caches: beyond the 256 MB of the Infinity Cache
 // nothing of it can be found there later.  Measured past / through: dropout 16384 x 8192 bf16 with
-// residual 131 / 157 us, without 91 / 94; gather of 65536 x 2048 bf16 99 / 125; combine of
-// 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16 (17 MB) 7.8 / 7.4; the reads of y of
-// the combine's gradient (16384 x 8 x 4096) 480 / 495.  Rows written for one read are slower past them
-// (dispatch 249 / 223, the gradient's writes 525 / 495).
+// residual 131 / 157 us, without 91 / 98; fp32 without 224 / 204, so that it goes through them; gather of
+// 65536 x 2048 bf16 99 / 125; combine of 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16
+// (17 MB) 7.8 / 7.4; the reads of y of the combine's gradient (16384 x 8 x 4096) 480 / 495.  Rows written
+// for one read are slower past them (dispatch 249 / 223, the gradient's writes 525 / 495).
 static bool past_caches(int64_t bytes) { return bytes > ((int64_t)256 << 20); }
 
 template <typename F>
@@ -1240,10 +1320,15 @@ static void by_flag(bool b, F f) {
     else f(std::false_type());
 }
 
-// lanes of a row of `cols` values, and the launch of `rows` such rows
+// Lanes of a row of `cols` values, and the launch of `rows` such rows.  256 lanes where two thirds of them
+// have work (dispatch and combine of 8 rows of 20000 tokens, 256 / 64 lanes: 1030 bf16 216 / 208 us, 1400
+// 226 / 273, 2047 of 16384 298 / 335) and the row has `wide` blocks of eight: gather's loads of its
+// indexes come before a row's values, and 64 lanes in steps wait for them once (65536 rows of 2047 bf16
+// 172 / 123, 2048 99 / 95, 1030 131 / 84).
 template <typename F>
-static void by_row(int64_t rows, int64_t cols, F f) {
-    const int L = cols <= 128 ? 16 : cols <= 1024 ? 64 : 256;
+static void by_row(int64_t rows, int64_t cols, int64_t wide, F f) {
+    const int64_t blocks = (cols + 7) / 8, all = (blocks + 255) / 256 * 256;
+    const int L = blocks <= 16 ? 16 : blocks <= 32 ? 32 : blocks < wide || 3 * blocks < 2 * all ? 64 : 256;
     int64_t x = (rows + 256 / L - 1) / (256 / L), y = 1;
     if (x < 2048) {      // few rows: their columns over several workgroups
         y = (cols + L * 8 - 1) / (L * 8);
@@ -1252,8 +1337,21 @@ static void by_row(int64_t rows, int64_t cols, F f) {
     }
     const dim3 grid((unsigned)(x < (1 << 20) ? x : 1 << 20), (unsigned)y);
     if (L == 16) f(std::integral_constant<int, 16>(), grid);
+    else if (L == 32) f(std::integral_constant<int, 32>(), grid);
     else if (L == 64) f(std::integral_constant<int, 64>(), grid);
     else f(std::integral_constant<int, 256>(), grid);
+}
+
+// The same where a row's lanes need not meet: rows of less than `narrow` values as one range of blocks.
+// Row by row / as one range: gather of 65536 rows of 130 bf16 24 / 17 us, 300 39 / 26, 515 51 / 35,
+// 1000 53 / 63;
+// combine of 8 rows of 72 of 466000 tokens 285 / 201, 130 of 258000 328 / 223, 200 of 168000 209 / 174,
+// 300 of 32768 (with its dispatch) 106 / 117.  Dispatch is no faster so (128: 134 / 150, 200: 188 / 197).
+template <typename F>
+static void by_block(int64_t rows, int64_t cols, int64_t narrow, int64_t wide, F f) {
+    if (cols >= narrow) return by_row(rows, cols, wide, f);
+    const int64_t x = (rows * ((cols + 7) / 8) + 255) / 256;
+    f(std::integral_constant<int, 0>(), dim3((unsigned)(x < 8192 ? x : 8192)));
 }
 
 template <typename F>
@@ -1273,10 +1371,13 @@ hipError_t launch_dropout(const void *x, int64_t ldx, const void *residual, int6
     const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_flag(past_caches(rows * cols * (int64_t)sizeof(T) * (residual ? 3 : 2)), [&](auto NT) {
+        by_flag((residual || sizeof(T) == 2) && past_caches(rows * cols * (int64_t)sizeof(T) * (residual ? 3 : 2)), [&](auto NT) {
             by_flag(residual != nullptr, [&](auto RES) {
-                hipLaunchKernelGGL((k_dropout<T, decltype(RES)::value, decltype(NT)::value>), grid, dim3(256), 0, s,
-                                   (const T *)x, ldx, (const T *)residual, ldr, (T *)y, rows, cols, (uint32_t)nb, d);
+                by_flag(cols % 8 == 0, [&](auto WHOLE) {
+                    hipLaunchKernelGGL((k_dropout<T, decltype(RES)::value, decltype(NT)::value, decltype(WHOLE)::value>),
+                                       grid, dim3(256), 0, s, (const T *)x, ldx, (const T *)residual, ldr, (T *)y, rows,
+                                       cols, (uint32_t)nb, d);
+                });
             });
         });
     });
@@ -1287,10 +1388,12 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
     if (rows <= 0 || cols <= 0) return hipSuccess;
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_row(rows, cols, [&](auto L, dim3 grid) {
+        by_block(rows, cols, 640, 257, [&](auto L, dim3 grid) {
             by_flag(past_caches(2 * rows * cols * (int64_t)sizeof(T)), [&](auto NT) {
-                hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value, decltype(NT)::value>), grid, dim3(256), 0, s,
-                                   (const T *)data, (T *)out, rows, cols, d, g);
+                by_flag(cols % 8 == 0, [&](auto WHOLE) {
+                    hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value, decltype(NT)::value, decltype(WHOLE)::value>),
+                                       grid, dim3(256), 0, s, (const T *)data, (T *)out, rows, cols, d, g);
+                });
             });
         });
     });
@@ -1354,7 +1457,7 @@ hipError_t launch_dispatch(const MoveArgs &m, const void *x, int64_t ldx, void *
     if (m.T <= 0 || m.D <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+        by_row(m.T, m.D, 0, [&](auto L, dim3 grid) {
             hipLaunchKernelGGL((k_dispatch<T, decltype(L)::value>), grid, dim3(256), 0, s, m, (const T *)x, ldx, (T *)xs);
         });
     });
@@ -1365,7 +1468,7 @@ hipError_t launch_combine(const MoveArgs &m, const void *y, const float *w, cons
     if (m.T <= 0 || m.D <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+        by_block(m.T, m.D, 257, 0, [&](auto L, dim3 grid) {
             by_slots(m.k < 8 ? m.k : 8, [&](auto KU) {
                 by_flag(past_caches(m.T * (m.k + 2) * m.D * (int64_t)sizeof(T)), [&](auto NT) {
                     hipLaunchKernelGGL((k_combine<T, decltype(L)::value, decltype(KU)::value, decltype(NT)::value>), grid,
@@ -1381,7 +1484,7 @@ hipError_t launch_combine_grad(const MoveArgs &m, const void *dout, int64_t ldo,
     if (m.T <= 0) return hipSuccess;
     return by_type(m.dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_row(m.T, m.D, [&](auto L, dim3 grid) {
+        by_row(m.T, m.D, 0, [&](auto L, dim3 grid) {
             grid.y = 1;     // the products run over all columns
             by_slots(m.k, [&](auto KM) {
                 by_flag(past_caches(m.T * (2 * m.k + 1) * m.D * (int64_t)sizeof(T)), [&](auto NT) {

@@ -462,6 +462,36 @@ def test_combine_gradients_one_at_a_time_and_strides():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [8, 9, 10, 11, 12, 13, 14, 15, 121, 129, 135, 255, 257, 263, 509, 513, 1023, 1031, 2055])
+def test_a_value_does_not_depend_on_the_width(dtype, D):
+    # the first D columns of rows of more of them: the same bits, but for the sums over a row
+    T, k, wide, kw = 37, 3, 2304, dict(p=0.3, key=11, rows=5)
+    r = plan_of(T, 8, k, D)
+    w = r.weights.detach().requires_grad_()
+    r = r._replace(weights=w)
+    x, res, dout = (rnd(i, T, wide, dtype=dtype) for i in (1, 2, 3))
+    ys = rnd(4, T * k, wide, dtype=dtype)
+    dout[:, D:] = 0
+
+    def passes(n):
+        y = ys[:, :n].contiguous().requires_grad_()
+        out = ops.combine(y, r, residual=res[:, :n], **kw)
+        dy, dw = torch.autograd.grad(out, (y, w), dout[:, :n])
+        a = x[:, :n].contiguous()
+        return dw, ops.dropout(a, 0.3, 11), ops.dropout(a, 0.3, 11, residual=res[:, :n]), ops.dispatch(a, r), \
+            ops.combine(y, r), out, dy
+
+    got, want = passes(D), passes(wide)
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a, b[:, :D])
+    # both sums: D roundings of products of g, y and 10/7
+    used = (r.experts >= 0)[..., None]
+    rows = torch.where(used, ys[:, :D].double()[r.pos.long()], 0.0)
+    mag = (dout[:, None, :D].double() * rows).abs().sum(2) * 65536 / 45875
+    assert ((got[0].double() - want[0].double()).abs() <= 2 * U * (wide + 4) * mag).all()
+
+
 def test_dispatch_past_2_31_values():
     T, k, D = 70000, 8, 4096                              # 2.3e9 values of expert-ordered rows
     r = ops.route(rnd(1, T, 16), k)
