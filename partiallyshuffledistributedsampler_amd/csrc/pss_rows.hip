@@ -617,7 +617,7 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
     __shared__ unsigned long long odd_rows, nan_rows;
     __shared__ __align__(16) uint16_t chosen[kRouteChunk * KP];
     __shared__ float2 stat[kRouteChunk];
-    __shared__ int wild;        // a bias is no number: groups are then summed by choose64 alone
+    __shared__ uint32_t steep;  // 1 + the largest |bias|, 0 without biases, as the bits of a float
     constexpr int kIndex = L * V <= 256 ? 8 : 10;
     constexpr uint32_t kIndexMask = (1u << kIndex) - 1, kExactMask = 0x1FFFu;
     const int E = a.E, k = a.k, G = a.groups, S = E / G;
@@ -637,18 +637,25 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
     for (int i = threadIdx.x; i < E; i += kThreads) mask[i] = 0;
     if (G > 1)
         for (int i = threadIdx.x; i < kThreads / L * Gp; i += kThreads) ((uint32_t *)room)[i] = 0;
-    if (threadIdx.x == 0) { odd_rows = nan_rows = 0; wild = 0; }
+    if (threadIdx.x == 0) { odd_rows = nan_rows = 0; steep = 0; }
     __syncthreads();
     // (in LDS, value v of lane x at v / 4 * 4 * L + 4 * x + v % 4: registers are what limits the waves)
     __shared__ float bias[L * V < 64 ? 64 : L * V];
     constexpr int kVec = V < 4 ? V : 4;
-    if (a.bias)
+    if (a.bias) {
+        float far = 0.f;
         for (int e = threadIdx.x; e < L * V; e += kThreads) {
             const int x = e / V, v = e % V;
             const float b = e < E ? a.bias[e] : 0.f;
             bias[(v / kVec * L + x) * kVec + v % kVec] = b;
-            if (G > 1 && !(fabsf(b) < 1e30f)) wild = 1;
+            // (a bias that is no number leaves every row's groups to choose64)
+            if (b != 0.f) far = fmaxf(far, fabsf(b) < 1e30f ? 1.f + fabsf(b) : INFINITY);
         }
+        if (G > 1) {
+            far = seg_max<64>(far);
+            if ((threadIdx.x & 63) == 0) atomicMax(&steep, __float_as_uint(far));
+        }
+    }
     auto add_bias = [&](float (&c)[V]) {
 #pragma unroll
         for (int v = 0; v < V; v++) c[v] += bias[(v / kVec * L + lane) * kVec + v % kVec];
@@ -697,7 +704,8 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
             if (a.bias) add_bias(c);
         }
         if (G > 1) {
-            odd |= wild != 0;
+            const float far = __uint_as_float(steep);
+            odd |= far >= 1e30f;
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = fmaxf(c[v], -INFINITY);      // (a median takes no NaN)
             // the two best of every group: a lane's values one by one, then across lanes, or through LDS
@@ -763,9 +771,11 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
             if (!exact) {
                 least = seg_reduce<L>(least, Min());
                 most = seg_reduce<L>(most, Max());
-                // two scores' errors on either side, and of the sums the roundings and the keys' 64 units
+                // two scores' errors on either side, of the sums the roundings and the keys' 64 units, and half a
+                // step of each of the four summands: biases of opposite sign leave a sum far below them
                 const float p = group_value(least), q = group_value(most);
-                if (most) odd |= !(p - q > 4.f * eps + 0x1.4p-17f * fmaxf(fabsf(p), fabsf(q))) && q > -INFINITY;
+                const float apart = 4.f * eps + (a.group_sum == 2 ? 0x1p-22f * far : 0.f) + 0x1.4p-17f * fmaxf(fabsf(p), fabsf(q));
+                if (most) odd |= !(p - q > apart) && q > -INFINITY;
             }
             wave_lds_sync();
             const uint32_t g0 = ((uint32_t)(lane * V) * inv) >> 20;

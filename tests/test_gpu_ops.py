@@ -327,6 +327,17 @@ def test_route_large_biases(bias, groups):
     check_route(rnd(3, 300, 60, dtype="bf16"), 5, bias=b, groups=groups, top_groups=max(1, groups // 2))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("G,S", [(2, 2), (2, 3), (4, 2)])
+@pytest.mark.parametrize("bias", [1e3, 1e4])
+def test_route_groups_whose_biases_cancel(score, G, S, bias):
+    # +B and -B in every group: a group's value is of the scores' size, its terms' rounding of the bias's
+    b = torch.full((G, S), -bias)
+    b[torch.arange(G), torch.arange(G) % S] = bias
+    l = rnd(G * S, 4000, G * S, scale=1e-3)
+    check_route(l, 1, score=score, bias=b.reshape(-1).to(dev()), groups=G, top_groups=1, group_sum=2)
+
+
 def test_plan_that_route_did_not_make_writes_nowhere_else():
     T, k, D = 6, 2, 40
     r = ops.route(rnd(1, T, 4), k)
