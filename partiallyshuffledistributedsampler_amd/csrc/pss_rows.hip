@@ -1080,10 +1080,11 @@ __global__ __launch_bounds__(kGradThreads) void k_route_grad(RouteArgs a, const 
                 sum += s[v];
             }
             sum = seg_reduce<L>(sum, Sum());
-            const float f = sum != 0.f ? dot / sum : 0.f;
+            // (a row without an expert has dot 0, and its logits may hold anything; else a NaN makes dot one)
+            const float f = dot != 0.f ? dot / sum : 0.f;
 #pragma unroll
             for (int v = 0; v < V; v++)
-                if (s[v] != 0.f) o[v] -= s[v] * f;
+                if (s[v] != 0.f && f != 0.f) o[v] -= s[v] * f;
         }
         if (row && lane * V < E) store(dlogits + t * E + lane * V, E - lane * V, o);
         wave_lds_sync();

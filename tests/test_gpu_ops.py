@@ -373,6 +373,32 @@ def test_route_strided_logits_and_no_gradient():
         assert not ops.route(leaf, 4).weights.requires_grad
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+@pytest.mark.parametrize("T,E", [(40, 20), (40, 300), (9000, 20)])
+def test_route_gradient_ignores_the_logits_of_padding(dtype, score, renormalise, T, E):
+    clean = rnd(T + E, T, E, dtype=dtype)
+    valid = torch.ones(T, dtype=torch.bool, device=dev())
+    valid[::3] = False
+    dirty = clean.clone()
+    dirty[0, 1], dirty[3, :] = float("nan"), float("nan")
+    dirty[6, 2], dirty[9, 3] = float("inf"), float("-inf")
+    dirty[12, 0], dirty[12, 1] = float("inf"), float("nan")
+    dirty[15, :] = float("-inf")
+    dw = rnd(7, T, 3)
+
+    def passes(l):
+        l = l.detach().requires_grad_()
+        r = ops.route(l, 3, score=score, renormalise=renormalise, valid=valid)
+        return tuple(r) + torch.autograd.grad(r.weights, l, dw)
+
+    got, want = passes(dirty), passes(clean)
+    assert (got[-1][::3] == 0).all()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(renormalise=False), dict(score="sigmoid"),
                                 dict(score="sigmoid", renormalise=False, scale=2.0)], ids=str)
 def test_route_gradient_against_differences(kw):
