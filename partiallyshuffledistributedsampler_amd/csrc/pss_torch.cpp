@@ -82,11 +82,16 @@ using Opt = std::optional<Tensor>;
 Opt opt(const Tensor &t) { return t.defined() ? Opt(t) : Opt(); }
 Tensor get(const Opt &t) { return t ? *t : Tensor(); }
 
+// The values as they lie in memory: torch may hold a sign that is still to be applied (the imaginary part of a
+// conjugate), which `contiguous` alone leaves as it is.
+Tensor plain(const Tensor &t) { return t.resolve_neg().contiguous(); }
+
 // Rows [.., D]: as they are where they lie at one distance and a row's values are adjacent, else copied.
 struct Rows {
     Tensor t;
     int64_t n, d, ld;
-    explicit Rows(const Tensor &x) {
+    explicit Rows(const Tensor &x_) {
+        const Tensor x = x_.resolve_neg();
         if (x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1)) {
             t = x;
             n = x.size(0);
@@ -122,7 +127,7 @@ variable_list once(const variable_list &in, variable_list out) {
 Tensor dropout_run(const Tensor &x, const Tensor &residual, double p, uint64_t key, int64_t row0, const Tensor &ids) {
     const Rows r(x);
     Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    Rows q(residual.defined() ? residual : r.t);
+    const Rows q(residual.defined() ? residual : r.t);
     const bool host = x.is_cpu();
     c10::OptionalDeviceGuard guard;
     if (!host) guard.reset_device(x.device());
@@ -189,7 +194,7 @@ Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Te
                       files, " files");
     Tensor out = get(out_), ids = get(ids_);
     if (out.defined()) {
-        TORCH_CHECK_VALUE(out.is_contiguous() && out.scalar_type() == data.scalar_type() && out.device() == device &&
+        TORCH_CHECK_VALUE(out.is_contiguous() && !out.is_neg() && out.scalar_type() == data.scalar_type() && out.device() == device &&
                               out.numel() >= n * values,
                           "gather: out must be contiguous, of the data's dtype, on the engine's device");
     } else {
@@ -199,7 +204,8 @@ Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Te
     }
     check_ids(ids, n, data);
     if (ids.defined()) ids = ids.reshape({-1}).contiguous();
-    check(lib.pss_gather_dropout((pss_sampler *)handle, data.const_data_ptr(), dtype_of(data), values,
+    const Tensor rows = data.resolve_neg();
+    check(lib.pss_gather_dropout((pss_sampler *)handle, rows.const_data_ptr(), dtype_of(data), values,
                                  base.const_data_ptr<int64_t>(), fpos.const_data_ptr<int32_t>(),
                                  off.const_data_ptr<int32_t>(), n, p, key, row0, ids_ptr(ids), ids_n(ids),
                                  out.data_ptr(), data.is_cpu() ? nullptr : stream_of(data)),
@@ -247,7 +253,7 @@ struct Route : torch::autograd::Function<Route> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &experts = saved[1], &weights = saved[2], &slopes = saved[3];
         const int64_t n = experts.size(0), k = experts.size(1), e = ctx->saved_data["experts"].toInt();
-        const Tensor dw = g[1].contiguous();
+        const Tensor dw = plain(g[1]);
         c10::DeviceGuard guard(dw.device());
         out[0] = at::empty({n, e}, weights.options().dtype((at::ScalarType)ctx->saved_data["dtype"].toInt()));
         const Rows r(saved[0].defined() ? saved[0] : out[0]);
@@ -276,7 +282,7 @@ variable_list route(const Tensor &logits, int64_t k, int64_t score, const Opt &b
         TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->device() == logits.device() && bias->dim() == 1 &&
                               bias->size(0) == e,
                           "bias must be float32 [", e, "] on the logits' device");
-        b = bias->detach().contiguous();
+        b = plain(bias->detach());
     }
     if (valid) {
         TORCH_CHECK_VALUE(valid->scalar_type() == at::kBool && valid->device() == logits.device() && valid->dim() == 1 &&
@@ -299,11 +305,11 @@ std::pair<int64_t, int64_t> check_plan(const Tensor &experts, const Tensor &pos,
 
 Tensor combine_run(const Tensor &y_, const Tensor &experts, const Tensor &pos, const Tensor &w, const Tensor &residual,
                    double p, uint64_t key, int64_t row0, const Tensor &ids) {
-    const Tensor y = y_.contiguous();
+    const Tensor y = plain(y_);
     const int64_t n = pos.size(0), k = pos.size(1), d = y.size(1);
     c10::DeviceGuard guard(y.device());
     Tensor out = at::empty({n, d}, y.options());
-    Rows q(residual.defined() ? residual : y);
+    const Rows q(residual.defined() ? residual : y);
     check(lib.pss_combine(y.const_data_ptr(), n, (int32_t)k, d, dtype_of(y), experts.const_data_ptr<int32_t>(),
                           pos.const_data_ptr<int32_t>(), (const float *)ptr(w),
                           residual.defined() ? q.t.const_data_ptr() : nullptr, q.ld, p, key, row0, ids_ptr(ids),
@@ -350,7 +356,7 @@ struct Combine : torch::autograd::Function<Combine> {
         const bool want_y = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         if (want_y || want_w) {
             const auto saved = ctx->get_saved_variables();
-            const Tensor y = saved[0].contiguous(), &w = saved[1], &experts = saved[2], &pos = saved[3], &ids = saved[4];
+            const Tensor y = plain(saved[0]), &w = saved[1], &experts = saved[2], &pos = saved[3], &ids = saved[4];
             const Rows r(g[0]);
             const int64_t n = pos.size(0), k = pos.size(1);
             c10::DeviceGuard guard(y.device());
@@ -393,7 +399,7 @@ Tensor combine(const Tensor &y, const Tensor &weights, const Tensor &experts, co
         check_ids(*ids, n, y);
         i = ids->reshape({-1}).contiguous();
     }
-    return Combine::apply(y, weights.contiguous(), residual, experts, pos, p, (int64_t)key, row0, opt(i));
+    return Combine::apply(y, plain(weights), residual, experts, pos, p, (int64_t)key, row0, opt(i));
 }
 
 }  // namespace

@@ -544,6 +544,33 @@ def test_dispatch_past_2_31_values():
     del xs, out
 
 
+def test_values_whose_sign_torch_still_holds():
+    # contiguous views with the sign as a bit, in the place of every tensor of values
+    T, E, k, D = 9, 6, 2, 24
+
+    def neg(seed, *shape):
+        v = torch._neg_view(rnd(seed, *shape))
+        assert v.is_neg()
+        return v, v.clone()
+
+    l, b, x, y, res, w = (neg(i, *s) for i, s in enumerate([(T, E), (E,), (T, D), (T * k, D), (T, D), (T, k)]))
+    r = ops.route(rnd(9, T, E), k)
+    dw, dout = neg(10, T, k), neg(11, T, D)
+    dxs = neg(12, T * k, D)
+
+    def passes(i):
+        ll, xx, yy, ww = (t[i].detach().requires_grad_() for t in (l, x, y, w))
+        q = ops.route(ll, k, bias=b[i], score="sigmoid", renormalise=False)
+        xs = ops.dispatch(xx, r)
+        out = ops.combine(yy, r._replace(weights=ww), residual=res[i], p=0.3, key=2)
+        full = ops.route(ll, k, renormalise=False)
+        return tuple(q) + (xs, out) + torch.autograd.grad((q.weights, full.weights, xs, out), (ll, xx, yy, ww),
+                                                          (dw[i], dw[i], dxs[i], dout[i]))
+
+    for a, c in zip(passes(0), passes(1)):
+        assert torch.equal(a, c)
+
+
 # ---- together ------------------------------------------------------------------------------------
 def layer(x, router, w1, p, key, rows, k=2):
     """A layer of experts: route, dispatch, each expert's product, combine."""

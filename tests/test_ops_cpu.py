@@ -86,6 +86,35 @@ def test_dropped_values_are_zero_whatever_they_were():
     assert torch.equal(ops.dropout(x, 1.0, 11), torch.zeros(8, 32))
 
 
+@pytest.mark.parametrize("shape", [(6, 1), (1, 6), (6, 5), (1,), (7,)])
+def test_values_whose_sign_torch_still_holds(shape):
+    # the imaginary part of a conjugate: a view of the positive values with a bit for the sign
+    z = torch.randn(*shape, 2, generator=torch.Generator().manual_seed(len(shape)))
+    v = torch.view_as_complex(z).conj().imag
+    want = v.clone()
+    assert v.is_neg() and not want.is_neg() and torch.equal(v, want)
+    x = torch.randn(shape)
+    assert torch.equal(ops.dropout(v, 0.3, 5), ops.dropout(want, 0.3, 5))
+    assert torch.equal(ops.dropout(x, 0.3, 5, residual=v), ops.dropout(x, 0.3, 5, residual=want))
+    x.requires_grad_()
+    r = x.detach().clone().requires_grad_()
+    got, both = (torch.autograd.grad(ops.dropout(x, 0.3, 5, residual=r), (x, r), g) for g in (v, want))
+    for a, b in zip(got, both):
+        assert torch.equal(a, b)
+
+
+def test_gather_of_values_whose_sign_torch_still_holds():
+    flat = torch._neg_view(torch.randn(22, 5, generator=torch.Generator().manual_seed(2)))
+    eng = IndexEngine([5, 3, 9, 1, 4], 22, 1, 4, 1, seed=5, device="cpu")
+    eng.init_iter(2)
+    fpos, off = eng.generate_mapped(0, 1)
+    base = torch.tensor([0, 5, 8, 17, 18])
+    assert flat.is_neg() and flat.is_contiguous()
+    assert torch.equal(eng.gather(flat, base, fpos, off, p=0.3, key=4), eng.gather(flat.clone(), base, fpos, off, p=0.3, key=4))
+    with pytest.raises(ValueError, match="out must be"):
+        eng.gather(flat, base, fpos, off, p=0.3, out=torch._neg_view(torch.empty(22, 5)))
+
+
 def test_keep_rate_and_key_separation():
     n, p = 1 << 18, 0.25
     a = ops.dropout(torch.ones(64, n // 64), p, ops.dropout_key(1, 2, 3, 4)) != 0
