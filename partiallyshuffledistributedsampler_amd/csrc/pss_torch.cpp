@@ -10,7 +10,9 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/pss.h"
 
@@ -42,6 +44,19 @@ void check(int rc, const char *name) {
 
 void *stream_of(const Tensor &t) {
     return (void *)at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+
+// The entries work on memory, which a recorder of torch's own operations does not see: its graph would hold
+// the allocation of an output and nothing that fills it.  (torch.compile runs these calls outside its graphs.)
+void check_eager() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    const bool recorded = torch::jit::tracer::isTracing() ||
+                          c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                          TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+                          TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) ||
+                          TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL);
+    TORCH_CHECK(!recorded, "the batch-row operators cannot be traced, exported or run on fake tensors");
 }
 
 // ---- arguments -----------------------------------------------------------------------------------
@@ -125,6 +140,7 @@ variable_list once(const variable_list &in, variable_list out) {
 
 // ---- dropout -------------------------------------------------------------------------------------
 Tensor dropout_run(const Tensor &x, const Tensor &residual, double p, uint64_t key, int64_t row0, const Tensor &ids) {
+    check_eager();
     const Rows r(x);
     Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     const Rows q(residual.defined() ? residual : r.t);
@@ -179,6 +195,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t key, int64_t row0, const Opt 
 Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Tensor &data, const Tensor &base_rows_,
               const Tensor &fpos_, const Tensor &off_, const Opt &out_, double p, uint64_t key, int64_t row0,
               const Opt &ids_) {
+    check_eager();
     check_p(p);
     TORCH_CHECK_TYPE(dtype_of(data) >= 0, "gather with dropout needs float32, bfloat16 or float16 data, got ",
                      data.scalar_type());
@@ -218,6 +235,7 @@ struct Route : torch::autograd::Function<Route> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, int64_t k, int64_t score, const Opt &bias,
                                  const Opt &valid, int64_t groups, int64_t top_groups, int64_t group_sum, bool renorm,
                                  double scale) {
+        check_eager();
         const Rows r(logits);
         const auto i32 = logits.options().dtype(at::kInt);
         c10::DeviceGuard guard(logits.device());
@@ -250,6 +268,7 @@ struct Route : torch::autograd::Function<Route> {
     static variable_list backward(AutogradContext *ctx, variable_list g) {
         variable_list out(10);
         if (!g[1].defined() || !ctx->needs_input_grad(0)) return out;
+        check_eager();
         const auto saved = ctx->get_saved_variables();
         const Tensor &experts = saved[1], &weights = saved[2], &slopes = saved[3];
         const int64_t n = experts.size(0), k = experts.size(1), e = ctx->saved_data["experts"].toInt();
@@ -305,6 +324,7 @@ std::pair<int64_t, int64_t> check_plan(const Tensor &experts, const Tensor &pos,
 
 Tensor combine_run(const Tensor &y_, const Tensor &experts, const Tensor &pos, const Tensor &w, const Tensor &residual,
                    double p, uint64_t key, int64_t row0, const Tensor &ids) {
+    check_eager();
     const Tensor y = plain(y_);
     const int64_t n = pos.size(0), k = pos.size(1), d = y.size(1);
     c10::DeviceGuard guard(y.device());
@@ -320,6 +340,7 @@ Tensor combine_run(const Tensor &y_, const Tensor &experts, const Tensor &pos, c
 
 struct Dispatch : torch::autograd::Function<Dispatch> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &experts, const Tensor &pos) {
+        check_eager();
         const Rows r(x);
         const int64_t k = pos.size(1);
         c10::DeviceGuard guard(x.device());
@@ -355,6 +376,7 @@ struct Combine : torch::autograd::Function<Combine> {
         if (!g[0].defined()) return out;
         const bool want_y = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         if (want_y || want_w) {
+            check_eager();
             const auto saved = ctx->get_saved_variables();
             const Tensor y = plain(saved[0]), &w = saved[1], &experts = saved[2], &pos = saved[3], &ids = saved[4];
             const Rows r(g[0]);

@@ -571,6 +571,26 @@ def test_values_whose_sign_torch_still_holds():
         assert torch.equal(a, c)
 
 
+def test_recorders_of_torch_operations_are_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    l, x = rnd(1, 6, 8).requires_grad_(), rnd(2, 6, 16).requires_grad_()
+    r = ops.route(l, 2)
+    plan = r._replace(weights=r.weights.detach())       # (torch refuses a closure over what has a gradient itself)
+    y = rnd(3, 12, 16)
+    calls = [(lambda v: ops.route(v, 2).weights, l.detach()), (lambda v: ops.dispatch(v, plan), x.detach()),
+             (lambda v: ops.combine(v, plan), y)]
+    xs = ops.dispatch(x, r)
+    for f, v in calls:
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(v)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, v, check_trace=False)
+    for out, leaf in ((r.weights, l), (xs, x), (ops.combine(y, r), l)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(lambda g: torch.autograd.grad(out, leaf, g, retain_graph=True))(torch.ones_like(out))
+    assert torch.equal(ops.dispatch(x, r), xs)
+
+
 # ---- together ------------------------------------------------------------------------------------
 def layer(x, router, w1, p, key, rows, k=2):
     """A layer of experts: route, dispatch, each expert's product, combine."""

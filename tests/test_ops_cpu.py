@@ -115,6 +115,60 @@ def test_gather_of_values_whose_sign_torch_still_holds():
         eng.gather(flat, base, fpos, off, p=0.3, out=torch._neg_view(torch.empty(22, 5)))
 
 
+def test_recorders_of_torch_operations_are_refused():
+    # a recorded graph would hold an output's allocation and nothing that fills it
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(4, 8)
+    leaf = x.clone().requires_grad_()
+    y = ops.dropout(leaf, 0.5, 1)
+    eng = IndexEngine([4, 3], 7, 1, 4, 1, seed=5, device="cpu")
+    eng.init_iter(0)
+    fpos, off = eng.generate_mapped(0, 1)
+    data, base = torch.randn(7, 3), torch.tensor([0, 4])
+
+    class Model(torch.nn.Module):
+        def forward(self, v):
+            return ops.dropout(v, 0.5, 1)
+
+    def fake():
+        with FakeTensorMode():
+            return ops.dropout(torch.randn(4, 8), 0.5, 1)
+
+    calls = [lambda: make_fx(Model(), tracing_mode=m)(x) for m in ("real", "fake", "symbolic")]
+    calls += [
+        lambda: make_fx(Model(), pre_dispatch=True)(x),
+        lambda: torch.jit.trace(Model(), x, check_trace=False),
+        lambda: torch.export.export(Model(), (x,), strict=False),
+        fake,
+        lambda: make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True))(torch.ones(4, 8)),
+        lambda: make_fx(lambda d: eng.gather(d, base, fpos, off, p=0.5))(data),
+        lambda: torch.jit.trace(lambda d: eng.gather(d, base, fpos, off, p=0.5), data, check_trace=False),
+    ]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            call()
+    # calls around them still work
+    assert torch.equal(ops.dropout(x, 0.5, 1), y.detach())
+
+
+def test_dropout_in_a_compiled_function_and_in_a_checkpoint():
+    from torch.utils.checkpoint import checkpoint
+
+    x = torch.randn(4, 8, requires_grad=True)
+
+    def f(v):
+        return ops.dropout(v * 2, 0.5, 1) * 3
+
+    y = f(x)
+    want = torch.autograd.grad(y.sum(), x)
+    for g in (torch.compile(f, backend="eager"), lambda v: checkpoint(f, v, use_reentrant=False)):
+        z = g(x)
+        assert torch.equal(z, y)
+        assert torch.equal(torch.autograd.grad(z.sum(), x)[0], want[0])
+
+
 def test_keep_rate_and_key_separation():
     n, p = 1 << 18, 0.25
     a = ops.dropout(torch.ones(64, n // 64), p, ops.dropout_key(1, 2, 3, 4)) != 0
