@@ -260,9 +260,10 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
  *   logits themselves.
  *   weight = scale * s, over the sum of the chosen s if renorm (the bias is in no weight); scale is
  *   between 1e-18 and 1e18 in magnitude.
- *   A logit of -infinity masks the expert.  A row with fewer live experts than k has experts -1 and
- *   weights 0 at the end, a row with valid[t] == 0 in all slots (its logits are ignored).  A NaN
- *   counts as the lowest of all live choices, and the weights of its row are NaN.
+ *   A logit or a bias of -infinity masks the expert (a softmax still runs over it if only its bias is).
+ *   A row with fewer live experts than k has experts -1 and weights 0 at the end, a row with
+ *   valid[t] == 0 in all slots (its logits are ignored).  A choice value that is a NaN, of a logit or a
+ *   bias, counts as the lowest of all live ones; the weights of a row with a NaN logit are NaN.
  *   offsets[e] = rows of the experts before e, offsets[experts] = rows in all.  Slot s = t * k + j
  *   has the place pos[s] in the order by (expert, t); slots without an expert come after
  *   offsets[experts], in their own order; src is the inverse of pos.

@@ -372,7 +372,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // The choice of a row's experts from values in 64 bits, one at a time, by a whole wave: lane j's expert.
 // It is the definition of the choice, and what the 32-bit choice leaves to it where its values are too
 // close to tell the order, too far from the best, or no numbers.  l[v], bias[v]: of expert 64 * v + lane
-// (-inf past the last); m: the logits' maximum; sum: of their exponentials, set here if `exps`; value:
+// (l is -inf past the last, bias 0 without one); m: the logits' maximum; sum: of their exponentials, set here if `exps`; value:
 // E + G doubles of LDS (groups).  One row is 5 us of latency, which a launch sees once, at its end.
 template <int V>
 __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool exps, int lane, const float (&l)[V],
@@ -413,7 +413,7 @@ __device__ __forceinline__ int choose64(const RouteArgs &a, bool by_logit, bool 
             }
     }
 #pragma unroll
-    for (int v = 0; v < V; v++) c[v] = l[v] == -INFINITY ? kDead : c[v] >= kLast ? c[v] : kLast;
+    for (int v = 0; v < V; v++) c[v] = l[v] == -INFINITY || bias[v] == -INFINITY ? kDead : c[v] >= kLast ? c[v] : kLast;
     if (G > 1) {
         double *score = value + E;
 #pragma unroll

@@ -117,8 +117,9 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, top_groups=1, grou
     scale        factor of all weights (1e-18 to 1e18 in magnitude)
     valid        [T] bool: rows that are padding get no expert
 
-    The best choice first, ties to the lower index.  A logit of -inf masks the expert; a row with
-    fewer than k left has experts -1 and weights 0 in its last slots.  Gradients flow from
+    The best choice first, ties to the lower index.  A logit or a bias of -inf masks the expert; a row
+    with fewer than k left has experts -1 and weights 0 in its last slots.  A NaN is chosen last of all
+    that are not masked, and makes the weights NaN if it is a logit's.  Gradients flow from
     Routing.weights to the logits.  E <= 1024, k <= 16, groups <= 64, T < 2^28, T * k < 2^31."""
     if score not in SCORES:
         raise ValueError("score must be 'softmax' or 'sigmoid', got %r" % (score,))

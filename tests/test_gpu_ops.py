@@ -309,6 +309,22 @@ def test_route_of_nan_rows_stays_in_range(score, bias, groups):
     assert torch.equal(torch.sort(r.pos.reshape(-1))[0], torch.arange(48, dtype=torch.int32, device=dev()))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_nan_comes_last_of_what_is_not_masked(score):
+    nan, inf = float("nan"), float("inf")
+    b = torch.tensor([nan, 0.0, 0.25, -inf, 0.0, nan], device=dev())
+    l = torch.tensor([[9.0, 1.0, 1.0, 9.0, 3.0, 0.0], [9.0, -inf, 2.0, nan, 1.0, -inf], [-inf, -inf, -inf, 2.0, -inf, -inf]],
+                     device=dev())
+    r = ops.route(l, 6, score=score, bias=b)
+    assert r.experts[0].tolist() == [2, 4, 1, 0, 5, -1]
+    assert r.weights[0, :5].isfinite().all() and (r.weights[0, 5] == 0).all()
+    # (a softmax with a NaN logit has no number at all: the order of the indexes)
+    assert r.experts[1].tolist() == ([2, 4, 0, -1, -1, -1] if score == "sigmoid" else [0, 2, 4, -1, -1, -1])
+    assert r.weights[1, :3].isnan().all() and (r.weights[1, 3:] == 0).all()
+    assert r.experts[2].tolist() == [-1] * 6 and (r.weights[2] == 0).all()
+    assert r.offsets[-1] == 8
+
+
 def test_route_of_padding_alone_and_of_a_zero_router():
     for T, E, kw in ((300, 40, {}), (9, 7, dict(bias=torch.zeros(7, device=dev()))), (200, 300, dict(groups=4, top_groups=2))):
         l = rnd(T, T, E)
@@ -336,6 +352,25 @@ def test_route_groups_whose_biases_cancel(score, G, S, bias):
     b[torch.arange(G), torch.arange(G) % S] = bias
     l = rnd(G * S, 4000, G * S, scale=1e-3)
     check_route(l, 1, score=score, bias=b.reshape(-1).to(dev()), groups=G, top_groups=1, group_sum=2)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,E,k,kw", [
+    (50, 12, 4, {}), (50, 12, 11, {}), (300, 40, 6, dict(groups=5, top_groups=2, group_sum=2)),
+    (300, 40, 6, dict(groups=5, top_groups=4)), (40, 300, 16, dict(groups=60, top_groups=30, group_sum=2)),
+    (9000, 24, 3, dict(groups=6, top_groups=3, group_sum=2, renormalise=False))], ids=str)
+def test_route_bias_of_minus_infinity_masks_its_expert(dtype, score, T, E, k, kw):
+    b = rnd(E, E, scale=0.1)
+    b[::3] = float("-inf")
+    if "groups" in kw:
+        b[:E // kw["groups"]] = float("-inf")           # a whole group
+    r = check_route(rnd(T, T, E, dtype=dtype), k, score=score, bias=b, **kw)
+    masked = torch.isneginf(b).nonzero().flatten()
+    assert not torch.isin(r.experts, masked).any()
+    b[:] = float("-inf")
+    r = check_route(rnd(T, T, E, dtype=dtype), k, score=score, bias=b, **kw)
+    assert (r.experts == -1).all() and (r.weights == 0).all()
 
 
 def test_plan_that_route_did_not_make_writes_nowhere_else():
