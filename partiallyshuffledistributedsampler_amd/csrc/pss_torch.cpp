@@ -191,7 +191,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t key, int64_t row0, const Opt 
 }
 
 // ---- gather with dropout -------------------------------------------------------------------------
-// Rows of device-resident files (IndexEngine.gather with p > 0): `device` is the handle's.
+// Rows of device-resident files (IndexEngine.gather with p > 0): `device` is the handle's.  No autograd node.
 Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Tensor &data, const Tensor &base_rows_,
               const Tensor &fpos_, const Tensor &off_, const Opt &out_, double p, uint64_t key, int64_t row0,
               const Opt &ids_) {
@@ -201,6 +201,9 @@ Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Te
                      data.scalar_type());
     TORCH_CHECK_VALUE(data.device() == device && data.is_contiguous() && data.dim() > 0,
                       "gather: data must be contiguous rows on the engine's device");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(data.requires_grad() || (out_ && out_->requires_grad())),
+                "gather has no gradient: data and out must not require one (index the rows and call ops.dropout, or "
+                "gather under torch.no_grad)");
     const Tensor fpos = fpos_.reshape({-1}).contiguous(), off = off_.reshape({-1}).to(at::kInt).contiguous();
     const Tensor base = base_rows_.to(device, at::kLong).contiguous();
     const int64_t n = fpos.numel(), values = data.size(0) ? data.numel() / data.size(0) : 0;
@@ -227,6 +230,7 @@ Tensor gather(uint64_t handle, const at::Device &device, int64_t files, const Te
                                  off.const_data_ptr<int32_t>(), n, p, key, row0, ids_ptr(ids), ids_n(ids),
                                  out.data_ptr(), data.is_cpu() ? nullptr : stream_of(data)),
           "pss_gather_dropout");
+    if (out_ && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();     // (written in place)
     return out;
 }
 

@@ -166,7 +166,8 @@ class IndexEngine:
         samples, file f starting at row base_rows[f] (dataset order); returns data rows of the
         (file_pos, offset) pairs, in their order (the on-GPU form of V1:243-248).
         p > 0: the rows (float32, bfloat16 or float16) with dropout, in the same pass
-        (pss_gather_dropout) -- exactly ops.dropout(rows flattened to [n, values], p, key, rows)."""
+        (pss_gather_dropout) -- the values of ops.dropout(rows flattened to [n, values], p, key, rows).
+        The gather has no gradient; with p > 0, data that requires one is refused."""
         if p:
             from . import ops
             return ops.gather(self, data, base_rows, fpos, off, out, stream, p, key, rows)

@@ -201,6 +201,31 @@ def test_gather_with_dropout_is_gather_then_dropout(dtype):
         eng.gather(data, base, fpos, off, p=0.5, rows=torch.zeros(7, dtype=torch.int64))
 
 
+def test_gather_with_dropout_has_no_gradient_and_says_so():
+    eng = IndexEngine([5, 3], 8, 1, 4, 1, seed=5, device="cpu")
+    eng.init_iter(2)
+    fpos, off = eng.generate_mapped(0, 1)
+    base = torch.tensor([0, 5])
+    data = torch.randn(8, 6)
+    leaf, out = data.clone().requires_grad_(), torch.zeros(8, 6)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        eng.gather(leaf, base, fpos, off, p=0.3)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        eng.gather(data, base, fpos, off, p=0.3, out=out.clone().requires_grad_())
+    want = eng.gather(data, base, fpos, off, p=0.3)
+    with torch.no_grad():
+        got = eng.gather(leaf, base, fpos, off, p=0.3)
+    assert torch.equal(got, want) and not got.requires_grad
+    # an output that a graph has saved: its backward pass refuses what was written over it
+    x = torch.randn(8, 6, requires_grad=True)
+    y = (x * out).sum()
+    assert torch.equal(eng.gather(data, base, fpos, off, p=0.3, out=out), want)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        assert torch.equal(eng.gather(data, base, fpos, off, p=0.3, out=torch.empty(8, 6)), want)
+
+
 class _Files:
     def __init__(self, files):
         self.files = files
