@@ -569,7 +569,9 @@ __device__ __forceinline__ void place_chunk(const RouteArgs &a, int64_t t0, int 
 
 // Weight of the slot of a thread, KP threads a row: e its expert (0xFFFF: none); m, sum: the row's softmax
 // statistics (scores not renormalised).  Softmax is exp(l - max) / sum, renormalised over the chosen
-// alone; the ratio of the chosen sigmoids comes from their logarithms, which neither under- nor overflow.
+// alone; so are sigmoids, exp(min(l, 0)) / (1 + exp(-|l|)), with the best one's exp(min(l, 0)) taken out of
+// all: neither under- nor overflows.  k values a row, so the library's expf (fast_exp is off by 60 u at
+// 87 below the best).
 template <int KP>
 __device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i, int j, int e, bool nan, float m,
                                             float sum, uint64_t *mask) {
@@ -577,15 +579,12 @@ __device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i
     const float lw = used ? one_logit(a, t, e) : -INFINITY;
     float w = 0.f;
     if (a.renorm) {
-        // (the logarithm is off by 2^-24 absolutely: its argument is in [1, 2])
-        const float z = !used ? -INFINITY : a.score == 0 ? lw
-                        : fminf(lw, 0.f) - 0.69314718f * __builtin_amdgcn_logf(1.f + fast_exp(-fabsf(lw)));
-        const float zm = seg_max<KP>(z);
-        w = used ? fast_exp(z - zm) : 0.f;
+        const float best = seg_max<KP>(lw);
+        if (used) w = a.score == 0 ? expf(lw - best) : expf(fminf(lw, 0.f) - fminf(best, 0.f)) / (1.f + expf(-fabsf(lw)));
         const float ws = seg_reduce<KP>(w, Sum());
         w = used ? w / ws * a.scale : 0.f;
     } else if (used) {
-        w = a.scale * (a.score == 0 ? fast_exp(lw - m) / sum : 1.f / (1.f + fast_exp(-lw)));
+        w = a.scale * (a.score == 0 ? expf(lw - m) / sum : 1.f / (1.f + expf(-lw)));
     }
     if (used && nan) w = NAN;
     if (j < a.k) {
@@ -593,7 +592,7 @@ __device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i
         a.experts[slot] = used ? e : -1;
         a.weights[slot] = w;
         // 1 - sigmoid, for the gradient: its rows would else be read again for k values each
-        if (a.slopes) a.slopes[slot] = used ? 1.f / (1.f + fast_exp(lw)) : 0.f;
+        if (a.slopes) a.slopes[slot] = used ? 1.f / (1.f + expf(lw)) : 0.f;
         if (used) atomicOr((unsigned long long *)&mask[e], 1ull << i);
     }
 }

@@ -282,6 +282,47 @@ def test_route_extreme_logits(dtype):
     assert torch.allclose(w.sum(1), torch.ones(2, device=dev())) and (w > 0.2).all()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("E", [8, 60, 300])
+def test_route_weights_far_below_the_best(dtype, E):
+    # The exponents are exact.  expf is within 2 u; the row's sum, of 1 and terms below 5e-5, goes through
+    # at most 8 additions in a lane and 6 across lanes, u each; the quotient and the scale are u each: 18 u
+    l = torch.full((E, E), -100.0)
+    at = torch.arange(E)
+    far = -(10.0 + at * 77.0 / E).floor()               # -10 .. -87
+    l[:, 0] = 0.0
+    l[at[1:], at[1:]] = far[1:]
+    l = l.to(DT[dtype]).to(dev())
+    ld = f64(l)
+    for renorm in (False, True):
+        r = ops.route(l, 2, renormalise=renorm)
+        w = np.exp(ld)
+        w = w / (w.sum(1, keepdims=True) if not renorm else np.sort(w, 1)[:, -2:].sum(1, keepdims=True))
+        want = np.take_along_axis(w, r.experts.long().cpu().numpy(), 1)[1:]
+        off = np.abs(f64(r.weights)[1:] / want - 1)
+        assert (off <= 18 * U).all(), off.max() / U
+
+
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_route_sigmoid_weights_far_below_the_best(renormalise):
+    # expf within 2 u, a sum, a quotient (renormalised: two of each) and the scale 1 u each
+    n = 78
+    l = torch.stack([torch.zeros(n), -torch.arange(10.0, 10 + n)], 1).to(dev()).requires_grad_()
+    for shift in (0.0, -60.0 if renormalise else 0.0, 60.0 if renormalise else 0.0):
+        ls = (l.detach() + shift).requires_grad_()
+        r = ops.route(ls, 2, score="sigmoid", renormalise=renormalise)
+        s = R.scores(f64(ls), "sigmoid")
+        want = s / s.sum(1, keepdims=True) if renormalise else s
+        off = np.abs(f64(r.weights) / want - 1)
+        assert (off <= 10 * U).all(), off.max() / U
+    # and 1 - s of the gradient, where s is 1 in 32 bits
+    up = (-l.detach()).requires_grad_()
+    d, = torch.autograd.grad(ops.route(up, 1, score="sigmoid", renormalise=False).weights.sum(), up)
+    want = R.scores(-f64(up)[:, 1], "sigmoid") * R.scores(f64(up)[:, 1], "sigmoid")
+    off = np.abs(f64(d)[:, 1] / want - 1)
+    assert (off <= 12 * U).all(), off.max() / U
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("groups", [1, 4])
