@@ -67,9 +67,14 @@ class Routing(NamedTuple):
 
 
 def dropout_key(seed, epoch, rank=0, site=0):
-    """The 64-bit dropout key of one logical rank's epoch at one place (`site`) of a model."""
+    """The 64-bit dropout key of one logical rank's epoch at one place (`site`) of a model.  The seed is
+    taken modulo 2^64; epoch fits 64 bits, rank and site 32, with a sign."""
+    epoch, rank, site = int(epoch), int(rank), int(site)
+    for name, n, bits in (("epoch", epoch, 63), ("rank", rank, 31), ("site", site, 31)):
+        if not -(1 << bits) <= n < 1 << bits:
+            raise ValueError("%s must fit %d bits, got %d" % (name, bits + 1, n))
     v = ctypes.c_uint64()
-    _lib.call("pss_dropout_key", int(seed) & _MASK64, int(epoch), int(rank), int(site), ctypes.byref(v))
+    _lib.call("pss_dropout_key", int(seed) & _MASK64, epoch, rank, site, ctypes.byref(v))
     return v.value
 
 

@@ -169,6 +169,18 @@ def test_dropout_in_a_compiled_function_and_in_a_checkpoint():
         assert torch.equal(torch.autograd.grad(z.sum(), x)[0], want[0])
 
 
+def test_dropout_keys_of_numbers_that_do_not_fit():
+    # a wider number must not give the key of another place, rank or epoch
+    for kw, name in ((dict(site=1 << 31), "site"), (dict(site=-(1 << 31) - 1), "site"), (dict(rank=1 << 32), "rank"),
+                     (dict(epoch=1 << 63), "epoch"), (dict(epoch=1 << 64), "epoch")):
+        with pytest.raises(ValueError, match=name):
+            ops.dropout_key(**dict(dict(seed=1, epoch=2), **kw))
+    ends = [dict(site=(1 << 31) - 1), dict(site=-(1 << 31)), dict(rank=(1 << 31) - 1), dict(rank=-1), dict(epoch=(1 << 63) - 1),
+            dict(epoch=-(1 << 63)), dict(epoch=2)]
+    assert len({ops.dropout_key(**dict(dict(seed=1, epoch=2), **kw)) for kw in ends}) == len(ends)
+    assert ops.dropout_key(5 - (1 << 64), 2) == ops.dropout_key(5, 2)
+
+
 def test_keep_rate_and_key_separation():
     n, p = 1 << 18, 0.25
     a = ops.dropout(torch.ones(64, n // 64), p, ops.dropout_key(1, 2, 3, 4)) != 0
