@@ -101,6 +101,13 @@ Tensor get(const Opt &t) { return t ? *t : Tensor(); }
 // conjugate), which `contiguous` alone leaves as it is.
 Tensor plain(const Tensor &t) { return t.resolve_neg().contiguous(); }
 
+// Rows of [.., D], also where D is 0
+int64_t rows_of(const Tensor &x) {
+    int64_t n = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); i++) n *= x.size(i);
+    return n;
+}
+
 // Rows [.., D]: as they are where they lie at one distance and a row's values are adjacent, else copied.
 struct Rows {
     Tensor t;
@@ -115,7 +122,7 @@ struct Rows {
         } else {
             t = x.contiguous();
             d = x.dim() ? x.size(-1) : 1;
-            n = d ? x.numel() / d : 0;
+            n = rows_of(x);
             ld = d;
         }
     }
@@ -184,7 +191,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t key, int64_t row0, const Opt 
     if (residual) check_like("residual", *residual, x, x.sizes());
     Tensor i;
     if (ids) {
-        check_ids(*ids, x.size(-1) ? x.numel() / x.size(-1) : 0, x);
+        check_ids(*ids, rows_of(x), x);
         i = ids->reshape({-1}).contiguous();
     }
     return Dropout::apply(x, residual, p, (int64_t)key, row0, opt(i));

@@ -238,6 +238,17 @@ def test_gather_with_dropout_has_no_gradient_and_says_so():
         assert torch.equal(eng.gather(data, base, fpos, off, p=0.3, out=torch.empty(8, 6)), want)
 
 
+@pytest.mark.parametrize("shape", [(3, 0), (2, 3, 0), (0,), (0, 4), (2, 0, 4), (2, 0, 0)])
+def test_dropout_of_nothing_takes_its_rows_ids(shape):
+    x = torch.zeros(shape, requires_grad=True)
+    n = int(np.prod(shape[:-1]))
+    for rows in (5, torch.tensor([5]), torch.arange(n)):
+        y = ops.dropout(x, 0.5, 1, rows=rows, residual=x)
+        assert y.shape == shape and torch.autograd.grad(y.sum(), x)[0].shape == shape
+    with pytest.raises(ValueError, match="one id"):
+        ops.dropout(x, 0.5, 1, rows=torch.arange(n + 2))
+
+
 class _Files:
     def __init__(self, files):
         self.files = files
