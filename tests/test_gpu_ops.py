@@ -120,6 +120,30 @@ def test_gather_with_dropout(dtype, shape):
     eng.close()
 
 
+@pytest.mark.parametrize("dtype,rows,cols", [
+    ("bf16", 300, 2049), ("bf16", 300, 2056), ("fp32", 120, 4099), ("fp16", 2500, 2055), ("bf16", 40000, 2056),
+    ("fp32", 20000, 2051), ("bf16", 650000, 40), ("fp16", 560000, 33), ("fp32", 300000, 130)])
+def test_gather_with_dropout_of_wide_and_of_many_rows(dtype, rows, cols):
+    # wide rows, more bytes than the caches hold, and more blocks of eight than one pass of the workgroups
+    lens = [rows // 4, rows // 8, 1, rows - rows // 4 - rows // 8 - 1]
+    eng = IndexEngine(lens, rows, 1, 4096, 2, seed=5, device=0)
+    eng.init_iter(1)
+    fpos, off = eng.generate_mapped(0, 1)
+    base = torch.tensor(np.concatenate([[0], np.cumsum(lens)[:-1]]), device=dev())
+    data = torch.randn(rows, cols, device=dev(), dtype=torch.float32, generator=torch.Generator(dev()).manual_seed(cols)).to(DT[dtype])
+    got = eng.gather(data, base, fpos, off, p=0.3, key=42, rows=7)
+    plain = eng.gather(data, base, fpos, off)
+    order = torch.from_numpy(eng.file_order().astype(np.int64)).to(dev())
+    assert torch.equal(plain, data[base[order[fpos[0].long()]] + off[0].long()])
+    # the definition at the first, the last and some rows between
+    at = torch.cat([torch.arange(20), torch.arange(rows - 20, rows), torch.randint(0, rows, (60,), generator=torch.Generator().manual_seed(1))])
+    f = R.factor([7 + i for i in at.tolist()], cols, 0.3, 42)
+    v = f64(plain[at.to(dev())])
+    check(got[at.to(dev())], R.drop(v, f), DT[dtype], extra=U * np.abs(v * f))
+    assert torch.equal(got, ops.dropout(plain, 0.3, 42, rows=7))
+    eng.close()
+
+
 # ---- routing -------------------------------------------------------------------------------------
 def exponents(l, score):
     """[T, 1] the largest exponent that a row's weights go through: differences of logits (exp is 0
@@ -218,6 +242,25 @@ def test_route_of_many_rows_over_few_experts(E, k, kw, dtype):
     l = rnd(T + E, T, E, dtype=dtype, scale=2.0)
     g = torch.Generator().manual_seed(E)
     l = l.masked_fill(((torch.rand(T, 1, generator=g) < 0.1) & (torch.rand(T, E, generator=g) < 0.6)).to(dev()), float("-inf"))
+    check_route(l, k, valid=(torch.rand(T, generator=g) < 0.9).to(dev()), **kw)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("T,E,k,kw", [
+    (600, 300, 4, {}), (8300, 300, 8, {}), (8300, 520, 3, dict(score="sigmoid", bias=True)),
+    (700, 320, 6, dict(groups=10, top_groups=4, group_sum=2, score="sigmoid", bias=True, scale=2.5)),
+    (8200, 384, 8, dict(groups=12, top_groups=6, group_sum=2, renormalise=False)),
+    (8200, 512, 8, dict(groups=16, top_groups=4, score="sigmoid", renormalise=False)),
+    (530, 900, 16, dict(groups=10, top_groups=5, group_sum=2)), (530, 1000, 2, dict(groups=40, top_groups=9, bias=True))],
+    ids=str)
+def test_route_of_many_rows_over_many_experts(dtype, T, E, k, kw):
+    kw = dict(kw)
+    if kw.pop("bias", False):
+        kw["bias"] = rnd(4, E, scale=0.1)
+    l = rnd(T + E, T, E, dtype=dtype, scale=2.0)
+    g = torch.Generator().manual_seed(E)
+    l = l.masked_fill(((torch.rand(T, 1, generator=g) < 0.1) & (torch.rand(T, E, generator=g) < 0.6)).to(dev()), float("-inf"))
+    l[T // 2] = float("-inf")
     check_route(l, k, valid=(torch.rand(T, generator=g) < 0.9).to(dev()), **kw)
 
 
@@ -618,6 +661,42 @@ def test_dispatch_past_2_31_values():
     out = ops.combine(xs, r)                              # the weights of a row sum to 1
     assert (out[-100:].float() - x[-100:].float()).abs().max().item() <= 2 ** -8 * 6 * 1.01
     del xs, out
+
+
+@pytest.mark.parametrize("dtype,T,k,D", [
+    ("bf16", 300000, 8, 72), ("fp16", 270000, 2, 130), ("bf16", 20000, 4, 1024), ("bf16", 10000, 8, 1025),
+    ("fp32", 9000, 16, 520), ("bf16", 140000, 4, 4096)])
+def test_combine_and_gradients_of_many_rows(dtype, T, k, D):
+    # narrow rows of more blocks than one pass of the workgroups, more bytes than the caches hold, more
+    # than 2^31 values; the first, the last and some rows between against the definition
+    gen = torch.Generator(dev()).manual_seed(D)
+
+    def big(*shape):
+        return torch.randn(*shape, device=dev(), generator=gen, dtype=torch.float32 if T * k * D < 1 << 30 else DT[dtype]).to(DT[dtype])
+
+    r = ops.route(rnd(3, T, 20, dtype="bf16"), k, valid=(torch.rand(T, generator=torch.Generator().manual_seed(2)) < 0.9).to(dev()))
+    w = r.weights.detach().requires_grad_()
+    r = r._replace(weights=w)
+    y, res, dout, x = big(T * k, D).requires_grad_(), big(T, D), big(T, D), big(T, D).requires_grad_()
+    out = ops.combine(y, r, residual=res, p=0.2, key=5, rows=11)
+    dy, dw = torch.autograd.grad(out, (y, w), dout)
+    xs = ops.dispatch(x, r)
+    dx, = torch.autograd.grad(xs, x, y.detach())
+    at = torch.cat([torch.arange(20), torch.arange(T - 20, T), torch.randint(0, T, (60,), generator=torch.Generator().manual_seed(1))])
+    a = at.to(dev())
+    f = R.factor([11 + i for i in at.tolist()], D, 0.2, 5)
+    used = (r.experts[a] >= 0).cpu().numpy()
+    pos, wd = r.pos[a].long(), f64(w[a])
+    rows = np.where(used[..., None], f64(y[pos]), 0.0)
+    parts = wd[..., None] * rows
+    G = R.drop(f64(dout[a]), f)
+    check(out[a], R.drop(parts.sum(1), f) + f64(res[a]), DT[dtype],
+          extra=U * ((k + 3) * np.abs(parts).sum(1) * f + 2 * np.abs(f64(res[a]))))
+    check(dx[a], rows.sum(1), DT[dtype], extra=U * k * np.abs(rows).sum(1))
+    want = np.where(used[..., None], wd[..., None] * G[:, None], 0.0)
+    check(dy[pos], want, DT[dtype], extra=3 * U * np.abs(want))
+    check(dw[a], (G[:, None] * rows).sum(2), torch.float32, extra=U * (D + 4) * (np.abs(G)[:, None] * np.abs(rows)).sum(2))
+    assert np.array_equal(f64(xs[pos]), np.where(used[..., None], f64(x[a])[:, None], 0.0))
 
 
 def test_values_whose_sign_torch_still_holds():
