@@ -143,12 +143,18 @@ size_t v1_exact_ws_bytes(const Geometry &g, int32_t nr, int64_t pos_lo, int64_t 
 hipError_t launch_v1_exact(const Geometry &g, const RankDesc *ranks, int32_t rank_lo, int32_t nr,
                            int64_t pos_lo, int64_t count, int64_t epoch, int64_t *out, void *ws,
                            hipStream_t s, const MapArgs *mapped = nullptr, uint32_t *slot = nullptr);
+// Epochs drawn by one launch, each into its slot.
+struct XAhead {
+    static constexpr int kMax = 8;
+    int32_t n;
+    int64_t epoch[kMax];
+    uint32_t *slot[kMax];
+};
 // a draw slot of a call's windows (0 bytes: none -- windows through HBM in several passes) and
 // the epochs the runtime draws ahead for it (as the V2 slots below)
 size_t v1_exact_slot_bytes(const Geometry &g, int64_t pos_lo, int64_t count);
 int v1_exact_lookahead_depth(const Geometry &g, int64_t pos_lo, int64_t count);
-hipError_t launch_v1_exact_draws(const Geometry &g, int64_t pos_lo, int64_t count, int64_t epoch,
-                                 uint32_t *slot, hipStream_t s);
+hipError_t launch_v1_exact_draws(const Geometry &g, int64_t pos_lo, int64_t count, const XAhead &a, hipStream_t s);
 
 // V2 in the reference's exact order (pss_v2exact.hip): shuffle_buffer < 2^30, ns < 2^31
 bool v2_exact_supported(const Geometry &g);
@@ -158,7 +164,7 @@ size_t v2_exact_ws_bytes(const Geometry &g, int32_t nr);
 // draws into its workspace's own slot)
 size_t v2_exact_slot_bytes(const Geometry &g);
 int v2_exact_lookahead_depth(const Geometry &g);   // epochs drawn ahead (0: none)
-hipError_t launch_v2_exact_draws(const Geometry &g, int64_t epoch, uint32_t *slot, hipStream_t s);
+hipError_t launch_v2_exact_draws(const Geometry &g, const XAhead &a, hipStream_t s);
 // V1's long windows drawn in the split form (pss_v2split.h; pss_v2exact.hip): false when the
 // workgroup form should run instead (scratch null: draws made ahead into a slot)
 bool v1x_draws_split(int64_t w_lo, uint32_t nj, uint32_t n_full, uint32_t n_last, uint32_t B, uint32_t nbk,

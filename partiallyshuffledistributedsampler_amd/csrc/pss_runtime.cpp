@@ -336,12 +336,16 @@ struct pss_sampler {
     // Exact-order draw lookahead: the reference's draws depend on the epoch and the windows alone
     // (V1:165-171; V2:107-109,147), so once pss_generate ran in exact order for consecutive
     // epochs of one call shape, the MT draws of the next epochs are made ahead into draw slots,
-    // each on its own side stream (a few long windows keep ~11 CUs busy for
-    // milliseconds: several epochs' draws run side by side).  The call of a prepared epoch only
-    // decodes (V2) / resolves (V1).  PSS_EXACT_LOOKAHEAD=0 turns it off.
-    static constexpr int kXSlots = 9;
+    // half the depth at a time in one launch (a few long windows keep ~11 CUs busy for milliseconds:
+    // several epochs' draws run side by side), on two side streams in turn.  Streams share four
+    // hardware queues: with one stream per slot the caller's kernels waited behind draws in their
+    // queue and draws behind each other (C5, consecutive epochs, depth 8: V2 4.13 -> 2.1 ms, V1 1.57 ->
+    // 0.87; with one stream 2.0 and 0.9, but 4.0 against 2.6 and 1.45 against 1.05 at depth 4).  The
+    // call of a prepared epoch only decodes (V2) / resolves (V1).  PSS_EXACT_LOOKAHEAD=0 turns it off.
+    static constexpr int kXSlots = pss::XAhead::kMax + 1;
     DevBuf<uint32_t> xslot[kXSlots];
-    hipStream_t xside[kXSlots] = {};
+    hipStream_t xside[2] = {};
+    int xturn = 0;
     hipEvent_t xev_done[kXSlots] = {};   // per slot: its last draws
     hipEvent_t xev_read[kXSlots] = {};   // per slot: the last decode that read it
     struct XKey {                        // what a slot's draws depend on besides the epoch
@@ -716,8 +720,9 @@ int pss_destroy(pss_sampler *h) {
         for (hipEvent_t e : h->ev_done) if (e) (void)hipEventDestroy(e);
         if (h->ev_shared) (void)hipEventDestroy(h->ev_shared);
         h->d_val2.release(); h->d_buf2.release(); h->d_val3.release(); h->d_buf3.release();
+        for (hipStream_t x : h->xside)
+            if (x) { (void)hipStreamSynchronize(x); (void)hipStreamDestroy(x); }
         for (int k = 0; k < pss_sampler::kXSlots; k++) {
-            if (h->xside[k]) { (void)hipStreamSynchronize(h->xside[k]); (void)hipStreamDestroy(h->xside[k]); }
             if (h->xev_done[k]) (void)hipEventDestroy(h->xev_done[k]);
             if (h->xev_read[k]) (void)hipEventDestroy(h->xev_read[k]);
             h->xslot[k].release();
@@ -943,7 +948,7 @@ bool exact_lookahead_on() {
 
 // Exact order: this epoch's decode (V2) / resolution (V1) from the draw slot a previous call
 // prepared (else drawing first); then, if the previous call was epoch - 1 of this shape, the
-// draws of the coming epochs into free slots on their side streams.
+// draws of the coming epochs into free slots on the side streams.
 int generate_exact(pss_sampler *h, const pss::Geometry &g, int32_t rank_lo, int32_t nr, int64_t pos_lo,
                    int64_t count, int64_t *out_dev, hipStream_t s, const pss::Marker &mk) {
     constexpr int NX = pss_sampler::kXSlots;
@@ -1007,48 +1012,62 @@ int generate_exact(pss_sampler *h, const pss::Geometry &g, int32_t rank_lo, int3
     // being drawn or read are released by a later call)
     for (int k = 0; k < NX; k++) {
         if (!h->xslot[k].p || h->xpend[k].valid || k == use || (k < cap_slots && depth > 0)) continue;
-        if (hipStreamQuery(h->xside[k]) == hipSuccess && hipEventQuery(h->xev_read[k]) == hipSuccess)
+        if (hipEventQuery(h->xev_done[k]) == hipSuccess && hipEventQuery(h->xev_read[k]) == hipSuccess)
             h->xslot[k].release();
     }
     (void)hipGetLastError();   // (a query's hipErrorNotReady)
     if (!sequential || depth <= 0) return PSS_OK;
-    auto prepare_slot = [&](int k, int64_t ep) -> hipError_t {
-        hipError_t r;
-        if (!h->xside[k]) {
-            if ((r = hipStreamCreateWithFlags(&h->xside[k], hipStreamNonBlocking)) != hipSuccess) return r;
-            if ((r = hipEventCreateWithFlags(&h->xev_done[k], PSS_LA_EVENT_FLAGS)) != hipSuccess) return r;
-            if ((r = hipEventCreateWithFlags(&h->xev_read[k], PSS_LA_EVENT_FLAGS)) != hipSuccess) return r;
-        }
-        if (h->xslot[k].n < sw) {   // grows once: after its last draws and its last reader
-            if ((r = hipStreamSynchronize(h->xside[k])) != hipSuccess) return r;
-            if ((r = hipEventSynchronize(h->xev_read[k])) != hipSuccess) return r;
-            if ((r = h->xslot[k].ensure(sw)) != hipSuccess) return r;
-        }
-        if ((r = hipStreamWaitEvent(h->xside[k], h->xev_read[k], 0)) != hipSuccess) return r;   // its last decode
-        r = v1 ? pss::launch_v1_exact_draws(g, pos_lo, count, ep, h->xslot[k].p, h->xside[k])
-               : pss::launch_v2_exact_draws(g, ep, h->xslot[k].p, h->xside[k]);
-        if (r != hipSuccess) return r;
-        return hipEventRecord(h->xev_done[k], h->xside[k]);
-    };
-    for (int d = 1; d <= depth && d < NX; d++) {
+    // the missing epochs, once they are half the depth (a launch's draws take as long for several
+    // epochs as for one) or the next one is among them
+    pss::XAhead a{};
+    int at[pss::XAhead::kMax];
+    bool next = false, taken[NX] = {};
+    for (int d = 1; d <= depth && a.n < pss::XAhead::kMax; d++) {
         bool queued = false;
         for (const auto &p : h->xpend) queued |= p.valid && p.key == key && p.epoch == e + d;
         if (queued) continue;
         int k = -1;
-        for (int j = 0; j < cap_slots && k < 0; j++) if (!h->xpend[j].valid && j != use) k = j;
+        for (int j = 0; j < cap_slots && k < 0; j++) if (!h->xpend[j].valid && j != use && !taken[j]) k = j;
         if (k < 0) break;
-        if (prepare_slot(k, e + d) != hipSuccess) {
-            (void)hipGetLastError();
-            h->xpend[k].valid = false;
-            if (h->xside[k]) (void)hipStreamSynchronize(h->xside[k]);
-            h->xslot[k].release();
-            (void)hipGetLastError();
-            h->x_failed = true;
-            return PSS_OK;
-        }
-        h->xpend[k] = {true, key, e + d};
-        h->st_x_made++;
+        taken[k] = true;
+        next |= d == 1;
+        at[a.n] = k;
+        a.epoch[a.n++] = e + d;
     }
+    if (a.n == 0 || (!next && 2 * a.n < depth)) return PSS_OK;
+    auto prepare = [&]() -> hipError_t {
+        hipError_t r;
+        hipStream_t &x = h->xside[h->xturn];
+        if (!x && (r = hipStreamCreateWithFlags(&x, hipStreamNonBlocking)) != hipSuccess) return r;
+        for (int i = 0; i < a.n; i++) {
+            const int k = at[i];
+            for (hipEvent_t *ev : {&h->xev_done[k], &h->xev_read[k]})
+                if (!*ev && (r = hipEventCreateWithFlags(ev, PSS_LA_EVENT_FLAGS)) != hipSuccess) return r;
+            if (h->xslot[k].n < sw) {   // grows once: after its last draws and its last reader
+                if ((r = hipEventSynchronize(h->xev_done[k])) != hipSuccess) return r;
+                if ((r = hipEventSynchronize(h->xev_read[k])) != hipSuccess) return r;
+                if ((r = h->xslot[k].ensure(sw)) != hipSuccess) return r;
+            }
+            a.slot[i] = h->xslot[k].p;
+            if ((r = hipStreamWaitEvent(x, h->xev_read[k], 0)) != hipSuccess) return r;   // its last decode
+            if ((r = hipStreamWaitEvent(x, h->xev_done[k], 0)) != hipSuccess) return r;   // (draws that were dropped)
+        }
+        r = v1 ? pss::launch_v1_exact_draws(g, pos_lo, count, a, x) : pss::launch_v2_exact_draws(g, a, x);
+        for (int i = 0; i < a.n && r == hipSuccess; i++) r = hipEventRecord(h->xev_done[at[i]], x);
+        h->xturn ^= 1;
+        return r;
+    };
+    if (prepare() != hipSuccess) {
+        (void)hipGetLastError();
+        for (hipStream_t x : h->xside)
+            if (x) (void)hipStreamSynchronize(x);
+        for (int i = 0; i < a.n; i++) h->xslot[at[i]].release();
+        (void)hipGetLastError();
+        h->x_failed = true;
+        return PSS_OK;
+    }
+    for (int i = 0; i < a.n; i++) h->xpend[at[i]] = {true, key, a.epoch[i]};
+    h->st_x_made += a.n;
     return PSS_OK;
 }
 
@@ -1168,8 +1187,9 @@ int pss_set_order_mode(pss_sampler *h, int32_t mode) {
     if (mode != h->order_mode && mode == PSS_ORDER_COUNTER && !h->cpu && h->dev_init) {
         // leaving the exact order: the draws made ahead and their slots go
         DeviceGuard dg(h->device);
+        for (hipStream_t x : h->xside)
+            if (x) PSS_HIP(hipStreamSynchronize(x));
         for (int k = 0; k < pss_sampler::kXSlots; k++) {
-            if (h->xside[k]) PSS_HIP(hipStreamSynchronize(h->xside[k]));
             if (h->xev_read[k]) PSS_HIP(hipEventSynchronize(h->xev_read[k]));
             h->xpend[k].valid = false;
             h->xslot[k].release();

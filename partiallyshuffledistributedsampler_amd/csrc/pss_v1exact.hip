@@ -240,15 +240,20 @@ __global__ __launch_bounds__(64) void k_v1x_draws32(Geometry g, V1xBig b, int64_
 }
 
 // The same draws with a workgroup per window (pss_mt.h mt_draws_wg): few, long windows (C5: 2^20
-// entries, ~12 per rank)
-__global__ __launch_bounds__(kMtWgThreads) void k_v1x_draws32_wg(Geometry g, V1xBig b, int64_t epoch) {
+// entries, ~12 per rank), of one epoch or of several at once (blockIdx.y)
+struct V1xDraws {
+    int64_t epoch[XAhead::kMax];
+    uint32_t *J[XAhead::kMax], *BCNT[XAhead::kMax];
+};
+__global__ __launch_bounds__(kMtWgThreads) void k_v1x_draws32_wg(Geometry g, V1xBig b, V1xDraws d) {
     __shared__ MtWgShared sh;
     const uint64_t job = b.j0 + blockIdx.x;
     const int64_t w = b.w_lo + (int64_t)(job % (uint64_t)b.nw);
     const int n = v1x_len(g, w);
     if (n <= 1) return;
-    uint32_t *jw = b.J + (size_t)blockIdx.x * b.B;
-    uint32_t *cnt = b.BCNT + (size_t)blockIdx.x * b.nbk;
+    const int64_t epoch = d.epoch[blockIdx.y];
+    uint32_t *jw = d.J[blockIdx.y] + (size_t)blockIdx.x * b.B;
+    uint32_t *cnt = d.BCNT[blockIdx.y] + (size_t)blockIdx.x * b.nbk;
     if (threadIdx.x < 64) mt_seed_int(sh.mt[0], w == 0 ? epoch : epoch + w * 10000);
     __syncthreads();
     mt_draws_wg(sh, 0, (uint32_t)(n - 1), [&](uint32_t d) { return (uint32_t)n - d; },
@@ -595,7 +600,7 @@ static size_t v1x_st_offset(int64_t jobs, int64_t W) {
     return ((size_t)jobs * (size_t)W * sizeof(uint16_t) + 15u) & ~(size_t)15u;
 }
 
-static hipError_t v1x_big_draws(const Geometry &g, const V1xBig &b, int64_t epoch, hipStream_t s);
+static hipError_t v1x_big_draws(const Geometry &g, const V1xBig &b0, const V1xDraws &d, int n, hipStream_t s);
 
 // the LDS path's draws: J (u16, W per window) then the windows' seeded MT states
 static void v1x_small_draws(const Geometry &g, int64_t w_lo, int64_t nw, int64_t epoch, uint32_t *dst,
@@ -634,7 +639,7 @@ size_t v1_exact_slot_bytes(const Geometry &g, int64_t pos_lo, int64_t count) {
 }
 
 // epochs drawn ahead: windows through HBM on a workgroup each (few, long: C5's 12 keep 12 CUs
-// busy for ~3 ms) 8 (C5 V1 exact 3.75 -> 1.12 ms per epoch); one-wave draws of many windows fill
+// busy for ~3 ms) 8 (C5 V1 exact 2.2 -> 0.87 ms per epoch); one-wave draws of many windows fill
 // the chip, and drawn ahead beside the resolution they slowed C2 from 0.40 to 0.80 ms: none.
 // At most 4 GiB of slots; none without a slot.
 int v1_exact_lookahead_depth(const Geometry &g, int64_t pos_lo, int64_t count) {
@@ -645,20 +650,23 @@ int v1_exact_lookahead_depth(const Geometry &g, int64_t pos_lo, int64_t count) {
     return cap < (size_t)want ? (int)cap : want;
 }
 
-hipError_t launch_v1_exact_draws(const Geometry &g, int64_t pos_lo, int64_t count, int64_t epoch,
-                                 uint32_t *slot, hipStream_t s) {
+hipError_t launch_v1_exact_draws(const Geometry &g, int64_t pos_lo, int64_t count, const XAhead &a, hipStream_t s) {
     const V1xSlot t = v1x_slot(g, pos_lo, count);
-    if (!t.ok || !slot) return hipErrorInvalidValue;
+    if (!t.ok) return hipErrorInvalidValue;
     if (!t.big) {
-        v1x_small_draws(g, t.w_lo, t.nw, epoch, slot, s);
+        for (int i = 0; i < a.n; i++) v1x_small_draws(g, t.w_lo, t.nw, a.epoch[i], a.slot[i], s);
         return hipGetLastError();
     }
     V1xBig b{};
     b.w_lo = t.w_lo; b.nw = t.nw; b.j0 = 0; b.B = (uint32_t)t.W; b.nbk = v1x_nbk(t.W);
     b.nj = (uint32_t)t.nw;
-    b.J = slot;
-    b.BCNT = slot + (size_t)b.nj * b.B;
-    return v1x_big_draws(g, b, epoch, s);
+    V1xDraws d{};
+    for (int i = 0; i < a.n; i++) {
+        d.epoch[i] = a.epoch[i];
+        d.J[i] = a.slot[i];
+        d.BCNT[i] = a.slot[i] + (size_t)b.nj * b.B;
+    }
+    return v1x_big_draws(g, b, d, a.n, s);
 }
 
 size_t v1_exact_ws_bytes(const Geometry &g, int32_t nr, int64_t pos_lo, int64_t count) {
@@ -673,10 +681,13 @@ size_t v1_exact_ws_bytes(const Geometry &g, int32_t nr, int64_t pos_lo, int64_t 
     return (size_t)pj * v1x_job_words(W) * sizeof(uint32_t);
 }
 
-// the draw stage of one pass (J and its bucket counts BCNT)
-static hipError_t v1x_big_draws(const Geometry &g, const V1xBig &b, int64_t epoch, hipStream_t s) {
-    hipError_t e = hipMemsetAsync(b.BCNT, 0, sizeof(uint32_t) * (size_t)b.nj * b.nbk, s);
-    if (e != hipSuccess) return e;
+// the draw stage of one pass (J and its bucket counts BCNT) of n epochs
+static hipError_t v1x_big_draws(const Geometry &g, const V1xBig &b0, const V1xDraws &d, int n, hipStream_t s) {
+    V1xBig b = b0;
+    for (int i = 0; i < n; i++) {
+        const hipError_t e = hipMemsetAsync(d.BCNT[i], 0, sizeof(uint32_t) * (size_t)b.nj * b.nbk, s);
+        if (e != hipSuccess) return e;
+    }
     // few windows: a workgroup per window's MT stream (PSS_V1X_DRAWS_WG=0 / 1 forces a form)
     static const int wg_env = [] {
         const char *e = getenv("PSS_V1X_DRAWS_WG");
@@ -686,12 +697,19 @@ static hipError_t v1x_big_draws(const Geometry &g, const V1xBig &b, int64_t epoc
     // a call's own single pass of few long windows: split over the chip (pss_v2split.h), the
     // scratch being the pass's S, H and PART (free until the partition runs; a slot drawn ahead
     // has none: b.S null)
-    if (b.S && b.j0 == 0 && (uint64_t)b.nj == (uint64_t)b.nw &&
+    if (b.S && n == 1 && b.j0 == 0 && (uint64_t)b.nj == (uint64_t)b.nw &&
         v1x_draws_split(b.w_lo, b.nj, (uint32_t)v1x_len(g, b.w_lo), (uint32_t)v1x_len(g, b.w_lo + b.nw - 1), b.B,
-                        b.nbk, epoch, b.J, b.BCNT, b.S, (size_t)3 * b.nj * b.B, wg, s))
+                        b.nbk, d.epoch[0], d.J[0], d.BCNT[0], b.S, (size_t)3 * b.nj * b.B, wg, s))
         return hipGetLastError();
-    if (wg) hipLaunchKernelGGL(k_v1x_draws32_wg, dim3(b.nj), dim3(kMtWgThreads), 0, s, g, b, epoch);
-    else hipLaunchKernelGGL(k_v1x_draws32, dim3(b.nj), dim3(64), 0, s, g, b, epoch);
+    if (wg) {
+        hipLaunchKernelGGL(k_v1x_draws32_wg, dim3(b.nj, (uint32_t)n), dim3(kMtWgThreads), 0, s, g, b, d);
+        return hipGetLastError();
+    }
+    for (int i = 0; i < n; i++) {
+        b.J = d.J[i];
+        b.BCNT = d.BCNT[i];
+        hipLaunchKernelGGL(k_v1x_draws32, dim3(b.nj), dim3(64), 0, s, g, b, d.epoch[i]);
+    }
     return hipGetLastError();
 }
 
@@ -735,7 +753,7 @@ static hipError_t launch_v1_exact_big(const Geometry &g, const RankDesc *ranks, 
             b.J = slot;
             b.BCNT = slot + (size_t)b.nj * B;
         } else {
-            e = v1x_big_draws(g, b, epoch, s);
+            e = v1x_big_draws(g, b, V1xDraws{{epoch}, {b.J}, {b.BCNT}}, 1, s);
             if (e != hipSuccess) return e;
         }
         hipLaunchKernelGGL(k_v1x_bscan, dim3(b.nj), dim3(kV1xScanNT), 0, s, g, b);

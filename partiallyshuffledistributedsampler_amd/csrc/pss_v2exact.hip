@@ -150,10 +150,11 @@ __global__ __launch_bounds__(64) void k_v2x_tail_draws(V2xGeo x, int64_t epoch, 
 // streams (C5: 2^20 steps each, ~11 per rank), which leave most of the chip idle for ~11 ms --
 // so the launch also carries the tail draws: blocks past the windows' run ten tail blocks each
 // (one per wave) on the CUs the streams do not use (C5: 1.96 ms of k_v2x_tail_draws hidden).
-__global__ __launch_bounds__(kMtWgThreads) void k_v2x_draws_wg(V2xGeo x, int64_t epoch, uint32_t jobs, uint64_t blk0,
-                                                              uint32_t nr, uint32_t tail_blocks,
-                                                              uint32_t *__restrict__ K1, uint32_t *__restrict__ K2) {
+// Several epochs' draws at once: first the windows of all of them, then the tails; a slot is K1 | K2.
+__global__ __launch_bounds__(kMtWgThreads) void k_v2x_draws_wg(V2xGeo x, XAhead a, uint32_t jobs, uint64_t blk0,
+                                                              uint32_t tail_blocks) {
     __shared__ MtWgShared sh;
+    const uint32_t nr = (uint32_t)a.n;
     const uint64_t b = blk0 + blockIdx.x;
     if (b >= (uint64_t)jobs * nr) {   // tail mode: wave w takes tail block 10 (b - windows) + w
         const uint32_t wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));   // (uniform)
@@ -162,13 +163,13 @@ __global__ __launch_bounds__(kMtWgThreads) void k_v2x_draws_wg(V2xGeo x, int64_t
         if (rl >= nr) return;
         static_assert(sizeof(sh.tw) + sizeof(sh.tw_pad) >= sizeof(uint32_t) * kMtN * kMtWgWaves,
                       "a tail wave's MT state in tw");
-        v2x_tail_block(x, epoch, rl, (uint32_t)(tb % tail_blocks) * 64u, K1, (uint32_t *)sh.tw + kMtN * wv);
+        v2x_tail_block(x, a.epoch[rl], 0, (uint32_t)(tb % tail_blocks) * 64u, a.slot[rl], (uint32_t *)sh.tw + kMtN * wv);
         return;
     }
     const uint32_t rl = (uint32_t)(b / jobs), job = (uint32_t)(b % jobs);
     if (job >= x.S) return;
-    uint32_t *k1 = K1 + (size_t)rl * x.ns;
-    uint32_t *k2 = K2 + (size_t)rl * x.T2;
+    const int64_t epoch = a.epoch[rl];
+    uint32_t *__restrict__ k1 = a.slot[rl], *__restrict__ k2 = k1 + x.ns;
     const uint32_t s = job;
     const uint32_t W = x.T - s * x.B < x.B ? x.T - s * x.B : x.B, t0 = s * x.B;
     if (threadIdx.x < 64) mt_seed_int(sh.mt[0], s == 0 ? epoch + 2 : epoch + (int64_t)(s - 1) * 10000);
@@ -1054,30 +1055,34 @@ size_t v2_exact_slot_bytes(const Geometry &g) {
     return v2x_slot_words(v2x_geo(g)) * sizeof(uint32_t);
 }
 
-// the draws of one epoch into a slot: the pool2 windows' k1 / k2 (seeded ahead, then one wave or
-// one workgroup per window) and the tail's first draws
-static void v2x_draws(const V2xGeo &x, int64_t epoch, uint32_t *slot, hipStream_t s) {
-    const uint32_t nr = 1;
-    uint32_t *K1 = slot, *K2 = slot + x.ns, *ST = K2 + x.T2;
+// the draws of each of a's epochs into its slot: the pool2 windows' k1 / k2 (seeded ahead, then one
+// wave or one workgroup per window) and the tail's first draws
+static void v2x_draws(const V2xGeo &x, const XAhead &a, hipStream_t s) {
     const uint32_t tail_blocks = (x.P + 63u) / 64u;
-    if (x.S) {
+    if (x.S && v2x_draws_wg((uint64_t)x.S, x.B)) {
         // few long windows (the streams alone do not fill the chip): a workgroup per stream, the
-        // tail draws riding along on the idle CUs
-        const bool wg = v2x_draws_wg((uint64_t)x.S * (uint64_t)nr, x.B);
-        const uint64_t wblocks = (uint64_t)x.S * (uint64_t)nr;
-        const uint64_t tblocks = wg ? ((uint64_t)tail_blocks * (uint64_t)nr + kMtWgWaves - 1) / kMtWgWaves : 0u;
-        if (!wg)   // (nr = 1: one decoded sequence; S < 2^31 / B windows, tail_blocks <= 2^24)
+        // tail draws riding along on the idle CUs; one launch for all epochs
+        const uint64_t wblocks = (uint64_t)x.S * (uint64_t)a.n;
+        const uint64_t tblocks = ((uint64_t)tail_blocks * (uint64_t)a.n + kMtWgWaves - 1) / kMtWgWaves;
+        v2x_launch_blocks(wblocks + tblocks, [&](uint64_t b0, uint32_t nb) {
+            hipLaunchKernelGGL(k_v2x_draws_wg, dim3(nb), dim3(kMtWgThreads), 0, s, x, a, x.S, b0, tail_blocks);
+        });
+        return;
+    }
+    for (int i = 0; i < a.n; i++) {
+        const int64_t epoch = a.epoch[i];
+        uint32_t *K1 = a.slot[i], *K2 = K1 + x.ns, *ST = K2 + x.T2;
+        if (x.S) {   // (S < 2^31 / B windows, tail_blocks <= 2^24)
             hipLaunchKernelGGL(k_v2x_seed, dim3(mt_seed_blocks(x.S) + tail_blocks), dim3(64), 0, s,
                                MtSeedSpec{epoch, 0, -1, 2, x.S}, ST, x, epoch, K1);
-        v2x_launch_blocks(wblocks + tblocks, [&](uint64_t b0, uint32_t nb) {
-            if (wg) hipLaunchKernelGGL(k_v2x_draws_wg, dim3(nb), dim3(kMtWgThreads), 0, s, x, epoch, x.S, b0,
-                                       nr, tail_blocks, K1, K2);
-            else hipLaunchKernelGGL(k_v2x_draws, dim3(nb), dim3(64), 0, s, x, x.S, b0, (const uint32_t *)ST, K1, K2);
-        });
-    } else {
-        v2x_launch_blocks((uint64_t)tail_blocks * (uint64_t)nr, [&](uint64_t b0, uint32_t nb) {
-            hipLaunchKernelGGL(k_v2x_tail_draws, dim3(nb), dim3(64), 0, s, x, epoch, tail_blocks, b0, K1);
-        });
+            v2x_launch_blocks(x.S, [&](uint64_t b0, uint32_t nb) {
+                hipLaunchKernelGGL(k_v2x_draws, dim3(nb), dim3(64), 0, s, x, x.S, b0, (const uint32_t *)ST, K1, K2);
+            });
+        } else {
+            v2x_launch_blocks(tail_blocks, [&](uint64_t b0, uint32_t nb) {
+                hipLaunchKernelGGL(k_v2x_tail_draws, dim3(nb), dim3(64), 0, s, x, epoch, tail_blocks, b0, K1);
+            });
+        }
     }
 }
 
@@ -1223,7 +1228,7 @@ bool v1x_draws_split(int64_t w_lo, uint32_t nj, uint32_t n_full, uint32_t n_last
 }
 
 // epochs drawn ahead: the few long windows of the workgroup form keep ~S CUs busy for
-// milliseconds, so several epochs' draws run side by side (8: C5 V2 exact 10.9 -> 3.4 ms per
+// milliseconds, so several epochs' draws run side by side (8: C5 V2 exact 4.1 -> 2.1 ms per
 // epoch); the one-wave form already fills the chip, and drawn ahead beside the decode it slowed
 // C2 from 0.83 to 1.19 ms (profiles/r05/ab_exact_tile.txt §7): none.  At most 4 GiB of slots.
 int v2_exact_lookahead_depth(const Geometry &g) {
@@ -1235,9 +1240,9 @@ int v2_exact_lookahead_depth(const Geometry &g) {
     return cap < (size_t)want ? (int)cap : want;
 }
 
-hipError_t launch_v2_exact_draws(const Geometry &g, int64_t epoch, uint32_t *slot, hipStream_t s) {
-    if (!v2_exact_supported(g) || !slot) return hipErrorInvalidValue;
-    v2x_draws(v2x_geo(g), epoch, slot, s);
+hipError_t launch_v2_exact_draws(const Geometry &g, const XAhead &a, hipStream_t s) {
+    if (!v2_exact_supported(g)) return hipErrorInvalidValue;
+    v2x_draws(v2x_geo(g), a, s);
     return hipGetLastError();
 }
 
@@ -1278,7 +1283,7 @@ static hipError_t v2x_pass(const Geometry &g, const V2xGeo &x, const RankDesc *r
         const size_t rest = v2x_rest_words(x);
         slot = ws + rest;
         // the decode's arrays are free until the tiles run: the split draws' scratch
-        if (!v2x_draws_split(x, epoch, slot, ws, rest, s)) v2x_draws(x, epoch, slot, s);
+        if (!v2x_draws_split(x, epoch, slot, ws, rest, s)) v2x_draws(x, XAhead{1, {epoch}, {slot}}, s);
     }
     uint32_t *K1 = slot, *K2 = slot + x.ns;
     uint32_t *V = ws;

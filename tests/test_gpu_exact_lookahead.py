@@ -76,6 +76,27 @@ def test_v1_consecutive_epochs_with_draws_made_ahead(B):
         assert stats["exact_made"] > 0 and stats["exact_used"] >= len(EPOCHS) - 3, stats
 
 
+@pytest.mark.parametrize("version,B", [(1, 1 << 17), (2, 1 << 16)])
+@pytest.mark.parametrize("depth", [1, 2, 3, 5, 8])
+def test_draws_are_made_for_several_epochs_at_once(version, B, depth):
+    """Half the depth at a time (one launch), the next epoch's without delay; every epoch still
+    equals the exact oracle at any depth, in order, after jumps and after a restart."""
+    lens, N, R = _shape(B)
+    eng = IndexEngine(lens, N, R, B, version, device=0, order="exact")
+    eng.set_lookahead(depth)
+    made, ahead = [], 0
+    for e in EPOCHS:
+        eng.init_iter(e)
+        eng.generate(0, R)
+        ahead = max(ahead, e)
+        if e > 0 and (ahead == e or 2 * (e + depth - ahead) >= depth):   # (epoch 0 is no one's next)
+            ahead = e + depth
+        made.append(ahead - 1 if ahead > e else 0)
+        assert eng.lookahead_stats()["exact_made"] == made[-1], (e, made)
+    eng.close()
+    _check_epochs(B, version, EPOCHS[:9] + [20, 21, 22, 5, 6, 7, 8], lookahead=(depth, 1 << 30, -1))
+
+
 def test_epoch_jumps_drop_the_prepared_draws():
     # 0, 1 (queues 2, 3), 5 (not 1 + 1: its own draws, the slots of 2, 3 dropped), 6, 7, 3, 4
     _check_epochs(1 << 16, 2, [0, 1, 5, 6, 7, 3, 4])
