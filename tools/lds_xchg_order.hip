@@ -2,7 +2,7 @@
 // the lanes exchanging one after another in ascending lane order (lane l gets what the highest
 // lower lane on that word wrote, the lowest gets the old word, the word ends with the highest
 // lane's value)?  Random slot patterns over several table sizes; counts mismatches against that
-// sequential model.  Build: hipcc --offload-arch=gfx950 -O3 -o build/lds_xchg_order tools/lds_xchg_order.hip
+// sequential model.  Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o build/lds_xchg_order tools/lds_xchg_order.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

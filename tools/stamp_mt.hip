@@ -1,7 +1,7 @@
 // stamp_mt.hip -- diagnostic: the workgroup MT draws of pss_mt.h built with -DPSS_MT_STAMPS on
 // C5-shaped V2 pool2 windows (W = P = 2^20, 88 streams); prints the per-round phase clocks.
 // Build (from the repo root):
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -DPSS_MT_STAMPS -Ipartiallyshuffledistributedsampler_amd/csrc \
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -DPSS_MT_STAMPS -Ipartiallyshuffledistributedsampler_amd/csrc \
 //     -o build/stamp_mt tools/stamp_mt.hip
 #include "../partiallyshuffledistributedsampler_amd/csrc/pss_mt.h"
 #include <cstdio>

@@ -8,7 +8,7 @@
 //   stamp_v2x alone <shift>   ... into the output buffer shifted by <shift> ids (address effects)
 // (-DPSS_DIAG_TILE_SWAP: block b replays tile b ^ 1, so that tile parity and XCD trade places)
 // Build (from the repo root; -DPSS_V2_SRC='"<path>"' stamps another copy of pss_v2.hip):
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -DPSS_STAMPS -DPSS_STAMPS_EMIT_ONLY \
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -DPSS_STAMPS -DPSS_STAMPS_EMIT_ONLY \
 //     -Ipartiallyshuffledistributedsampler_amd/csrc -o build/stamp_v2x tools/stamp_v2x.hip \
 //     partiallyshuffledistributedsampler_amd/csrc/pss_v2grp.hip
 #ifndef PSS_V2_SRC

@@ -8,7 +8,7 @@
 //                 self-scheduling: big chunks first, small ones at the end)
 // Each variant also reports the bytes every XCC wrote (per-wave XCC_ID) and the spread of wave
 // end times (s_memrealtime, 100 MHz).
-// Build: hipcc --offload-arch=gfx950 -O3 -o build/ubench_balance tools/ubench_balance.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o build/ubench_balance tools/ubench_balance.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

@@ -1,7 +1,7 @@
 // ubench_lds.hip -- throughput of LDS ops at random word addresses over a 4096-word table (the
 // V2 slot table shape): plain write, no-return max, returning max, exchange, read.  One
 // 256-thread workgroup per CU slot; reports G lane-ops/s per CU.
-// Build: hipcc --offload-arch=gfx950 -O3 -o build/ubench_lds tools/ubench_lds.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o build/ubench_lds tools/ubench_lds.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

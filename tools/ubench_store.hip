@@ -1,7 +1,7 @@
 // ubench_store.hip -- streaming-store bandwidth in the V2 emit layouts: 2048 single-wave
 // workgroups (LDS-padded to 8 per CU), each writing its own contiguous run of int64 ids,
 // 512 B per store instruction (dwordx2 per lane) vs 1 KB (dwordx4: two ids per lane), with and
-// without a little ALU work per id.  Build: hipcc --offload-arch=gfx950 -O3 -o build/ubench_store tools/ubench_store.hip
+// without a little ALU work per id.  Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o build/ubench_store tools/ubench_store.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

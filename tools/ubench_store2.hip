@@ -8,7 +8,7 @@
 //   persist_r  2048 one-wave blocks, each its own contiguous 390 KB run (the sampler kernels)
 //   persist_r4 the same with dwordx4 stores (2 per 256 ids)
 //   persist_r16 4096 / 8192 one-wave blocks (16 / 32 per CU), own runs
-// Build: hipcc --offload-arch=gfx950 -O3 -o build/ubench_store2 tools/ubench_store2.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o build/ubench_store2 tools/ubench_store2.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
