@@ -245,7 +245,8 @@ int pss_dropout_key(uint64_t seed, int64_t epoch, int32_t rank, int32_t site, ui
 int pss_dropout(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *y, int64_t rows, int64_t cols,
                 int32_t dtype, double p, uint64_t key, int64_t row0, const int64_t *row_ids, int64_t n_ids,
                 int32_t host, void *stream);
-/* pss_gather of rows of row_values values, dropped in the same pass. */
+/* pss_gather of rows of row_values values, dropped in the same pass.  The pairs are of the handle's current
+ * epoch, and the call is not made on a capturing stream (PSS_ENOTSUP): the tables change with the epoch. */
 int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int64_t row_values,
                        const int64_t *base_rows_dev, const int32_t *file_pos_dev, const int32_t *offset_dev, int64_t n,
                        double p, uint64_t key, int64_t row0, const int64_t *row_ids_dev, int64_t n_ids, void *out_dev,

@@ -1433,6 +1433,11 @@ int pss_gather_dropout(pss_sampler *h, const void *data_dev, int32_t dtype, int6
     }
     DeviceGuard dg(h->device);
     hipStream_t s = (hipStream_t)stream;
+    // a replay would read this epoch's file order from a table that later epochs write over
+    hipStreamCaptureStatus capture;
+    PSS_HIP(hipStreamIsCapturing(s, &capture));
+    if (capture != hipStreamCaptureStatusNone)
+        return fail(PSS_ENOTSUP, "a gather with dropout cannot be captured: the handle's tables change with the epoch");
     SharedUse su(h, s);
     rc = prepare_tables(h, s);
     if (rc) return rc;

@@ -164,10 +164,12 @@ class IndexEngine:
     def gather(self, data, base_rows, fpos, off, out=None, stream=None, p=0.0, key=0, rows=0):
         """Rows of device-resident files (pss_gather): data [rows, ...] holds every dataset file's
         samples, file f starting at row base_rows[f] (dataset order); returns data rows of the
-        (file_pos, offset) pairs, in their order (the on-GPU form of V1:243-248).
+        (file_pos, offset) pairs -- of the current epoch -- in their order (the on-GPU form of
+        V1:243-248).
         p > 0: the rows (float32, bfloat16 or float16) with dropout, in the same pass
         (pss_gather_dropout) -- the values of ops.dropout(rows flattened to [n, values], p, key, rows).
-        The gather has no gradient; with p > 0, data that requires one is refused."""
+        The gather has no gradient; with p > 0, data that requires one is refused, and so is a
+        call while a graph is captured (the handle's tables change with the epoch)."""
         if p:
             from . import ops
             return ops.gather(self, data, base_rows, fpos, off, out, stream, p, key, rows)

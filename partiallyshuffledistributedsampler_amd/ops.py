@@ -13,14 +13,13 @@ row's id a resumed run (state_dict) drops what the uninterrupted one would have 
 the batch size and the number of GPUs.
 
 Every call runs on the current stream of its tensors' device, allocates its outputs there and keeps
-nothing; calls can be captured into a graph (capture a backward pass only while no eager autograd
-graph of the same leaves is alive: torch ties a leaf's accumulation to the stream that it was first
-used on, and waiting for that stream ends a capture).  They work on memory: torch.compile runs them
-outside its graphs, and what records torch's own operations (jit.trace, make_fx, export, fake
-tensors) is refused.  fp32, bf16 and fp16 rows; sums and softmax statistics
-are held in 32 bits or more and rounded once.  Rows may be strided, values of a row are adjacent
-(any other layout is copied first).  CPU tensors: dropout alone (the CPU mode, the same bits);
-routing needs a ROCm GPU.
+nothing; the four calls above can be captured into a graph (capture a backward pass only while no
+eager autograd graph of the same leaves is alive: torch ties a leaf's accumulation to the stream that
+it was first used on, and waiting for that stream ends a capture).  They work on memory: torch.compile
+runs them outside its graphs, and what records torch's own operations (jit.trace, make_fx, export,
+fake tensors) is refused.  fp32, bf16 and fp16 rows; sums and softmax statistics are held in 32 bits
+or more and rounded once.  Rows may be strided, values of a row are adjacent (any other layout is
+copied first).  CPU tensors: dropout alone (the CPU mode, the same bits); routing needs a ROCm GPU.
 """
 import ctypes
 from typing import NamedTuple

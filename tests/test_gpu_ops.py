@@ -120,6 +120,24 @@ def test_gather_with_dropout(dtype, shape):
     eng.close()
 
 
+def test_gather_with_dropout_is_not_captured():
+    # a replay after later epochs would read a file order that is no longer there
+    lens = [50, 31, 97, 1, 41]
+    eng = IndexEngine(lens, 220, 1, 16, 2, seed=5, device=0)
+    base = torch.tensor(np.concatenate([[0], np.cumsum(lens)[:-1]]), device=dev())
+    data = rnd(1, 220, 24)
+    for epoch in (2, 3, 4):
+        eng.init_iter(epoch)
+        fpos, off = eng.generate_mapped(0, 1)
+        want = ops.dropout(eng.gather(data, base, fpos, off), 0.3, 42)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                eng.gather(data, base, fpos, off, p=0.3, key=42)
+        assert torch.equal(eng.gather(data, base, fpos, off, p=0.3, key=42), want)
+    eng.close()
+
+
 @pytest.mark.parametrize("dtype,rows,cols", [
     ("bf16", 300, 2049), ("bf16", 300, 2056), ("fp32", 120, 4099), ("fp16", 2500, 2055), ("bf16", 40000, 2056),
     ("fp32", 20000, 2051), ("bf16", 650000, 40), ("fp16", 560000, 33), ("fp32", 300000, 130)])
