@@ -1332,9 +1332,12 @@ static void by_flag(bool b, F f) {
 
 // Lanes of a row of `cols` values, and the launch of `rows` such rows.  256 lanes where two thirds of them
 // have work (dispatch and combine of 8 rows of 20000 tokens, 256 / 64 lanes: 1030 bf16 216 / 208 us, 1400
-// 226 / 273, 2047 of 16384 298 / 335) and the row has `wide` blocks of eight: gather's loads of its
-// indexes come before a row's values, and 64 lanes in steps wait for them once (65536 rows of 2047 bf16
-// 172 / 123, 2048 99 / 95, 1030 131 / 84).
+// 226 / 273, 2047 of 16384 298 / 335) and the row has `wide` blocks of eight.  Gather's loads of its
+// indexes come before a row's values, and 64 lanes in steps wait for them once, which is what counts for
+// the fewer bytes of 16-bit rows of up to 256 blocks (65536 rows of bf16, 256 / 64 lanes: 1368 88 / 79,
+// 1449 143 / 96, 1920 98 / 94, 2047 170 / 121, 2048 100 / 98; the one range that loses is 2000 to 2040 in
+// whole blocks, 104 / 121; from 2049 on even, 3584 162 / 177), not for 32 bits (32768 rows: 1536 87 / 97,
+// 1921 117 / 128, 2047 121 / 135, 2048 110 / 126, 4096 232 / 252).
 template <typename F>
 static void by_row(int64_t rows, int64_t cols, int64_t wide, F f) {
     const int64_t blocks = (cols + 7) / 8, all = (blocks + 255) / 256 * 256;
@@ -1398,7 +1401,7 @@ hipError_t launch_gather_dropout(const void *data, void *out, int64_t rows, int6
     if (rows <= 0 || cols <= 0) return hipSuccess;
     return by_type(dtype, [&](auto *p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        by_block(rows, cols, 640, 257, [&](auto L, dim3 grid) {
+        by_block(rows, cols, 640, sizeof(T) == 2 ? 257 : 0, [&](auto L, dim3 grid) {
             by_flag(past_caches(2 * rows * cols * (int64_t)sizeof(T)), [&](auto NT) {
                 by_flag(cols % 8 == 0, [&](auto WHOLE) {
                     hipLaunchKernelGGL((k_gather_drop<T, decltype(L)::value, decltype(NT)::value, decltype(WHOLE)::value>),
