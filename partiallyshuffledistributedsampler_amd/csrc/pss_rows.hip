@@ -1053,8 +1053,9 @@ __global__ __launch_bounds__(kGradThreads) void k_route_grad(RouteArgs a, const 
             e = a.experts[tt * k + lane];
             if (e >= 0) { w = a.weights[tt * k + lane]; g = dweights[tt * k + lane]; }
         }
-        const float dot = seg_reduce<L>(g * w, Sum());
-        float x = w * (a.renorm ? g - dot / a.scale : g);
+        // (w / scale is exactly 1 for the only expert of a renormalised row, whose gradient is exactly 0)
+        const float dot = seg_reduce<L>(g * (a.renorm ? w / a.scale : w), Sum());
+        float x = w * (a.renorm ? g - dot : g);
         if (a.score == 1 && e >= 0) x *= a.slopes[tt * k + lane];
 #pragma unroll
         for (int v = 0; v < V; v++) d[v * L + lane] = 0.f;

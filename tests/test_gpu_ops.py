@@ -536,6 +536,22 @@ def test_route_gradient_ignores_the_logits_of_padding(dtype, score, renormalise,
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("scale", [1.0, 2.5, 0.3])
+def test_route_gradient_of_an_only_expert_is_zero(score, scale):
+    # a renormalised weight of one expert is the scale, whatever the logit
+    l = rnd(3, 900, 20)
+    l[::2, 1:] = float("-inf")
+    l.requires_grad_()
+    for k in (1, 3):
+        r = ops.route(l, k, score=score, scale=scale)
+        d, = torch.autograd.grad(r.weights, l, rnd(4, 900, k))
+        one = (r.experts >= 0).sum(1) == 1
+        assert one.sum() == (900 if k == 1 else 450)
+        assert (r.weights[one][:, 0] == torch.tensor(scale, device=dev())).all() and (d[one] == 0).all()
+        assert k == 1 or (d[~one] != 0).any()
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(renormalise=False), dict(score="sigmoid"),
                                 dict(score="sigmoid", renormalise=False, scale=2.0)], ids=str)
 def test_route_gradient_against_differences(kw):
