@@ -71,9 +71,9 @@ __device__ __forceinline__ void store(T *p, int64_t left, const float (&v)[N]) {
 // Eight values of a row of D, from column c (a multiple of 8) on, 0 past the end.  A lane at the end reads
 // the row's last eight and shifts them down: every lane makes the same wide load and several rows' loads
 // stay on their way, where a branch that reads the end value by value waits for each (combine of 8 rows
-// of 4095 bf16 of 8194 tokens: 169 -> 113 us; dropout of 16386 x 8191 bf16: 156 -> 122).  raw8 is the load
+// of 4095 bf16 of 8194 tokens: 169 -> 112 us; dropout of 16386 x 8191 bf16: 156 -> 119).  raw8 is the load
 // (NT: nontemporal, past the caches), open8 the rest.  WHOLE (gather and dropout): D % 8 is 0, and
-// no branch stands between the load and the Philox block (gather of 65536 x 2048 bf16: 162 -> 99).
+// no branch stands between the load and the Philox block (a call of gather of 65536 x 2048 bf16: 162 -> 99).
 template <bool NT = false, bool WHOLE = false, typename T>
 __device__ __forceinline__ typename Pack<T, 8>::V raw8(const T *row, int64_t c, int64_t D) {
     typedef typename Pack<T, 8>::V V;
@@ -156,8 +156,8 @@ __device__ __forceinline__ void drop8(const Drop &d, const Draw &u, float (&v)[8
 // y = dropout(x) (+ residual).  Bound by memory: a value is read (twice with a residual) and written, and
 // 20 32 x 32-bit products per 8 values hide behind that.  One thread per block of 8 columns, over rows and
 // blocks as one range, so that odd widths leave no lanes idle; (row, block) are stepped, not divided.
-// 16384 x 8192 bf16: 133 us with a residual (6.1 TB/s), 91 without (5.9); x 8191, whose rows start at
-// any 2 bytes, 171 and 115; 4093 x 1537 fp32, from the Infinity Cache: 14 and 10.
+// 16384 x 8192 bf16: 135 us with a residual (6.0 TB/s), 91 without (5.9); x 8191, whose rows start at
+// any 2 bytes, 178 and 126; 4093 x 1537 fp32, from the Infinity Cache: 14 and 9.
 template <typename T, bool RES, bool NT, bool WHOLE>
 __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,
                                                  int64_t ldr, T *__restrict__ y, int64_t rows, int64_t cols,
@@ -599,7 +599,7 @@ __device__ __forceinline__ void finish_slot(const RouteArgs &a, int64_t t, int i
 
 // The choice of the experts and their weights.  Bound by vector instructions, about 1000 a wave and four
 // rows of 256 experts (a third of them scores, a quarter the sorting networks); k rounds of a maximum over
-// 64-bit values took 166 us where this takes 43 (65536 rows, 8 of 256 experts in 16 groups, sigmoid and
+// 64-bit values took 166 us where this takes 45 (65536 rows, 8 of 256 experts in 16 groups, sigmoid and
 // bias, bf16; reading the logits alone: 7).
 //
 // One workgroup routes a chunk of up to 64 rows, L lanes a row and V experts a lane.  The choice runs on
@@ -945,7 +945,7 @@ __global__ __launch_bounds__(kThreads, L == 64 ? 4 : 6) void k_route(RouteArgs a
 
 // Rows of every expert in the chunks before each chunk, and in all chunks: a workgroup takes 8 experts,
 // 128 threads of each over the chunks (two passes; the masks of the second come from L2).  Bound by the
-// latency of those passes: 5.5 us for 1024 chunks of 256 experts (2 MB), 4 for 256 of 60.
+// latency of those passes: 5.6 us for 1024 chunks of 256 experts (2 MB), 4 for 256 of 60.
 __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict__ mask, int32_t *__restrict__ before,
                                                      int32_t *__restrict__ total, int64_t chunks, int E) {
     __shared__ int32_t part[8][129];
@@ -980,7 +980,7 @@ __global__ __launch_bounds__(1024) void k_route_scan(const uint64_t *__restrict_
 }
 
 // Places of one chunk's slots: the chunk's masks and sums, one scan over the experts, then a popcount a
-// slot.  Bound by latency: 7.7 us for 65536 x 8 slots, 4 for 16381 x 4.  Without the sums of k_route_scan
+// slot.  Bound by latency: 8 us for 65536 x 8 slots, 4 for 16381 x 4.  Without the sums of k_route_scan
 // a workgroup counts all chunks itself.
 __global__ __launch_bounds__(kPlaceThreads) void k_route_place(RouteArgs a, const int32_t *__restrict__ before,
                                                                const int32_t *__restrict__ totals) {
@@ -1031,7 +1031,7 @@ __global__ __launch_bounds__(kPlaceThreads) void k_route_place(RouteArgs a, cons
 //   softmax, renormalised:  scale * a_i * (g_i - sum g_j * a_j) at the chosen
 //   sigmoid:                w_i * (1 - s_i) * g_i at the chosen (renormalised: g_i - sum g_j * a_j)
 // L lanes a row; the slots' values go through LDS to the lanes that store them, so that the row leaves in
-// wide stores.  Bound by writing every value, nearly all of them 0: 12.5 us for 65536 x 256 bf16 (33.6 MB).
+// wide stores.  Bound by writing every value, nearly all of them 0: 12.4 us for 65536 x 256 bf16 (33.6 MB).
 constexpr int kGradThreads = 512;
 template <typename T, int L, int V>
 __global__ __launch_bounds__(kGradThreads) void k_route_grad(RouteArgs a, const float *__restrict__ dweights,
@@ -1126,7 +1126,7 @@ __device__ __forceinline__ void each8(int64_t rows, int64_t cols, F f) {
 
 // out[r] = dropout(row base[order[f_r]] + off_r of the data).  Bound by memory, a row's index loads first:
 // they are the same for the lanes of a row (scalar loads), and rows of other waves cover them.
-// 65536 rows of 2048 bf16: 95 us (5.6 TB/s), of 2047 123.
+// 65536 rows of 2048 bf16: 88 us (6.1 TB/s), of 2047 112.
 template <typename T, int L, bool NT, bool WHOLE>
 __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data, T *__restrict__ out, int64_t rows,
                                                      int64_t cols, Drop d, RowGather g) {
@@ -1145,7 +1145,7 @@ __global__ __launch_bounds__(256) void k_gather_drop(const T *__restrict__ data,
 }
 
 // xs[pos[t, j]] = x[t].  Bound by the k writes of a row, which is read once (a gather by place would read
-// it k times).  16384 rows of 4096 bf16 to 8 experts each: 230 us (5.2 TB/s).
+// it k times).  16384 rows of 4096 bf16 to 8 experts each: 247 us (4.9 TB/s).
 template <typename T, int L>
 __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restrict__ x, int64_t ldx, T *__restrict__ xs) {
     const uint32_t places = (uint32_t)(m.T * m.k);
@@ -1165,8 +1165,8 @@ __global__ __launch_bounds__(256) void k_dispatch(MoveArgs m, const T *__restric
 
 // out[t] = residual[t] + dropout(sum of w[t, j] * y[pos[t, j]]), the gradient of k_dispatch without weights
 // and residual.  Bound by the reads of k rows: KU of them are on their way at a time, and the Philox block
-// is computed meanwhile.  16384 x 8 rows of 4096 bf16: 238 us (5.1 TB/s), with residual and dropout
-// 267; 8194 x 8 of 4095 113 (5.3).  A slot without an expert is read like any other (its place is a row of
+// is computed meanwhile.  16384 x 8 rows of 4096 bf16: 219 us (5.5 TB/s), with residual and dropout
+// 242; 8194 x 8 of 4095 112 (5.4).  A slot without an expert is read like any other (its place is a row of
 // y) and left out of the sum whatever it holds.
 template <typename T, int L, int KU, bool NT>
 __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict__ y, const float *__restrict__ w,
@@ -1210,7 +1210,7 @@ __global__ __launch_bounds__(256) void k_combine(MoveArgs m, const T *__restrict
 
 // One pass over g = dropout(dout): KU products with rows of y and KU rows of dy at a time.  The lanes
 // of a row hold partial products of all its slots; they are joined after the last column.  Bound by the
-// k rows read and k written of a row.  16384 x 8 x 4096 bf16: 482 us (4.7 TB/s; a plain copy 4.95).
+// k rows read and k written of a row.  16384 x 8 x 4096 bf16: 473 us (4.8 TB/s; a plain copy 4.95).
 template <typename T, int L, int KM, bool NT>
 __global__ __launch_bounds__(256) void k_combine_grad(MoveArgs m, const int32_t *__restrict__ experts,
                                                       const int32_t *__restrict__ places, const T *__restrict__ dout, int64_t ldo,
@@ -1318,7 +1318,7 @@ void by_width(int E, int64_t T, F f) {
 }  // namespace
 
 // Whether a pass over so many bytes goes past the caches: beyond the 256 MB of the Infinity Cache
-// nothing of it can be found there later.  Measured past / through: dropout 16384 x 8192 bf16 with
+// nothing of it can be found there later.  Measured past / through, in one run each: dropout 16384 x 8192 bf16 with
 // residual 131 / 157 us, without 91 / 98; fp32 without 224 / 204, so that it goes through them; gather of
 // 65536 x 2048 bf16 99 / 125; combine of 16384 x 8 x 4096 bf16 233 / 281; combine of 2039 x 3 x 1001 fp16
 // (17 MB) 7.8 / 7.4; the reads of y of the combine's gradient (16384 x 8 x 4096) 480 / 495.  Rows written
