@@ -139,7 +139,7 @@ def test_gather_with_dropout_is_not_captured():
 
 
 @pytest.mark.parametrize("dtype,rows,cols", [
-    ("bf16", 300, 2049), ("bf16", 300, 2056), ("fp32", 120, 4099), ("fp16", 2500, 2055), ("bf16", 40000, 2056),
+    ("fp32", 300, 1375), ("fp32", 300, 2048), ("fp16", 300, 1375), ("bf16", 300, 2047), ("bf16", 300, 2049), ("bf16", 300, 2056), ("fp32", 120, 4099), ("fp16", 2500, 2055), ("bf16", 40000, 2056),
     ("fp32", 20000, 2051), ("bf16", 650000, 40), ("fp16", 560000, 33), ("fp32", 300000, 130)])
 def test_gather_with_dropout_of_wide_and_of_many_rows(dtype, rows, cols):
     # wide rows, more bytes than the caches hold, and more blocks of eight than one pass of the workgroups
@@ -731,6 +731,19 @@ def test_combine_and_gradients_of_many_rows(dtype, T, k, D):
     check(dy[pos], want, DT[dtype], extra=3 * U * np.abs(want))
     check(dw[a], (G[:, None] * rows).sum(2), torch.float32, extra=U * (D + 4) * (np.abs(G)[:, None] * np.abs(rows)).sum(2))
     assert np.array_equal(f64(xs[pos]), np.where(used[..., None], f64(x[a])[:, None], 0.0))
+
+
+@pytest.mark.parametrize("T,D", [(5, 0), (0, 0), (0, 7)])
+def test_rows_without_values_and_no_rows(T, D):
+    r = ops.route(rnd(1, T, 4), 2)
+    w = r.weights.detach().requires_grad_()
+    r = r._replace(weights=w)
+    x, y, res = (torch.zeros(n, D, device=dev(), requires_grad=True) for n in (T, 2 * T, T))
+    xs, out = ops.dispatch(x, r), ops.combine(y, r, residual=res, p=0.5, key=1, rows=torch.arange(T, device=dev()))
+    assert xs.shape == (2 * T, D) and out.shape == (T, D)
+    dx, dy, dw, dres = torch.autograd.grad((xs, out), (x, y, w, res), (torch.zeros_like(xs), torch.zeros_like(out)))
+    assert dx.shape == x.shape and dy.shape == y.shape and dres.shape == res.shape and (dw == 0).all() and dw.shape == (T, 2)
+    assert ops.dropout(x, 0.5, 1, rows=torch.arange(T, device=dev())).shape == (T, D)
 
 
 def test_values_whose_sign_torch_still_holds():
